@@ -405,6 +405,85 @@ int nncf_amd_gptq_pack8(const void* codes, int codes_signed, int64_t out_feature
 int nncf_amd_gptq_dequant8(const int32_t* qweight, const int32_t* qzeros, const void* scales, int64_t in_features,
                            int64_t out_features, void* weight, int out_dtype, void* stream);
 
+/*
+ * Products with compressed weights: y = act(x W^T + bias) + residual, W [n, k] read as codes, scales and zero points and
+ * multiplied with the value that nncf_amd_decompress gives it in the activations' type (integer modes, NF4: fp16 scale;
+ * MXFP4: E8M0 scale bytes).  Sums, bias, activation and residual are fp32, rounded once into y.  The reference decompresses
+ * the whole weight on every read in front of a library product (src/nncf/torch/quantization/layers.py:1303-1460).
+ *   x          : [m, k] fp16 / bf16 (dtype), rows ldx elements apart
+ *   codes      : as nncf_amd_decompress takes them, [n, k] in memory; group_size along k, -1 = whole row
+ *   bias       : [n] in x's type, nullable
+ *   activation : 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu, 5 swiglu: rows [0, n / 2) of W are the gate, y has n / 2
+ *                columns silu(gate) * up
+ *   residual   : [m, width] in x's type, rows ldr apart, nullable
+ *   y          : [m, width], rows ldy apart;  z : [m, n] nullable, the sums with their bias in x's type (what the gradient of
+ *                the activation needs)
+ *   workspace  : nncf_amd_compressed_linear_workspace bytes, aligned to 16 (0: none needed)
+ */
+size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, int mode,
+                                            int64_t group_size);
+int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes,
+                               int mode, int64_t group_size, const void* scale, const uint8_t* zero_point,
+                               const void* bias, int activation, const void* residual, int64_t ldr, void* y, int64_t ldy,
+                               void* z, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * The same for a stack of experts' weights [experts, n, k] and rows in the order of their experts: expert e owns the rows
+ * [offsets[e], offsets[e + 1]) of y (int32 [experts + 1], on the device); rows behind offsets[experts] get zeros.
+ * slots (nullable, int32 [rows]): row r reads x at slots[r] / topk, x has `sources` rows; NULL: x has the rows' order.
+ * Values outside the buffers are held to their ends.
+ */
+size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, int64_t sources, int gathered, int64_t rows, int64_t n,
+                                        int64_t k, int mode, int64_t group_size, int64_t experts);
+int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int64_t sources, const int32_t* slots, int64_t topk,
+                           const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k, const void* codes,
+                           int mode, int64_t group_size, const void* scale, const uint8_t* zero_point, int activation,
+                           void* y, int64_t ldy, void* z, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * dx = dz W for either (offsets == NULL: experts is 1), dz [rows, n] in the activations' type, rows ldz apart; dx [rows, k] in
+ * that type or fp32 (dx_is_f32), rows ldx apart.
+ */
+size_t nncf_amd_linear_grad_input_workspace(const void* dz, int64_t ldz, int64_t rows, int64_t n, int64_t k,
+                                            int64_t experts);
+int nncf_amd_linear_grad_input(const void* dz, int dtype, int64_t ldz, const int32_t* offsets, int64_t experts,
+                               int64_t rows, int64_t n, int64_t k, const void* codes, int mode, int64_t group_size,
+                               const void* scale, const uint8_t* zero_point, void* dx, int64_t ldx, int dx_is_f32,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * dz = dy * act'(z) [m, n] in the activations' type with rows ldz apart (the columns behind n become zero), nullable; and
+ * dbias [n] = the sums of dz over the rows, in fp32 and in a fixed order, rounded once; nullable.  z may be NULL without an
+ * activation.  workspace: only for dbias.
+ */
+size_t nncf_amd_activation_grad_workspace(int64_t m, int64_t n);
+int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, const void* z, int64_t m, int64_t n, int activation,
+                             void* dz, int64_t ldz, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+/*
+ * Routing of tokens to experts: the topk largest logits of every row of [tokens, experts] (fp32 / fp16 / bf16, rows ldl
+ * apart), falling, ties to the lower number, NaN below every number; weights = their softmax (renormalize: over the chosen,
+ * else over all experts), fp32 [tokens, topk], 0 for a row of -inf.  ids, rows int32 [tokens, topk]; slots int32
+ * [tokens * topk]; offsets int32 [experts + 1]: the slots (token * topk + place) sorted stably by expert, rows[slot] the
+ * place of a slot in that order and slots[row] its inverse.  mask (nullable, one byte per token): 0 = the token has no
+ * experts: ids and rows -1, weights 0; slots behind the last row are -1.  experts <= 1024, topk <= 64.
+ */
+size_t nncf_amd_route_experts_workspace(int64_t tokens, int64_t experts, int64_t topk);
+int nncf_amd_route_experts(const void* logits, int dtype, int64_t ldl, int64_t tokens, int64_t experts, int64_t topk,
+                           int renormalize, const uint8_t* mask, float* weights, int32_t* ids, int32_t* rows,
+                           int32_t* slots, int32_t* offsets, void* workspace, size_t workspace_bytes, void* stream);
+/* dlogits [tokens, experts] (contiguous, the logits' type) from dweights fp32 [tokens, topk] and the call's results. */
+int nncf_amd_route_experts_grad(const void* logits, int dtype, int64_t ldl, int64_t tokens, int64_t experts, int64_t topk,
+                                int renormalize, const float* weights, const int32_t* ids, const float* dweights,
+                                void* dlogits, void* stream);
+/*
+ * out[t] = sum_j weights[t, j] * y[rows[t, j]] (weights NULL: plain sum; rows < 0 are left out), fp32 in the order of j,
+ * rounded once.  y [total_rows, n] in out's type or fp32, rows ldy apart; out [tokens, n] fp16 / bf16.
+ */
+int nncf_amd_combine_experts(const void* y, int in_dtype, int64_t ldy, int64_t total_rows, const float* weights,
+                             const int32_t* rows, int64_t tokens, int64_t topk, int64_t n, void* out, int out_dtype,
+                             void* stream);
+/* dy [tokens * topk, n] (nullable; zeros where slots[row] < 0) and dweights [tokens, topk] (nullable) from dout. */
+int nncf_amd_combine_experts_grad(const void* dout, int dtype, const void* y, int64_t ldy, const float* weights,
+                                  const int32_t* rows, const int32_t* slots, int64_t tokens, int64_t topk, int64_t n,
+                                  void* dy, float* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

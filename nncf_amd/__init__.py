@@ -6,6 +6,9 @@ from nncf_amd.parameters import (AdvancedAWQParameters, AdvancedCompressionParam
                                  AdvancedScaleEstimationParameters, BackupMode, CompressedWeight, CompressWeightsMode,
                                  Dataset, GroupSizeFallbackMode, IgnoredScope, SensitivityMetric,
                                  WeightCompressionConfig)
+from nncf_amd.experts import (CompressedExperts, ExpertRouting, combine_experts, compress_experts,  # noqa: F401
+                              expert_linear, route_experts)
+from nncf_amd.linear import compressed_linear, fuse_compressed_linears  # noqa: F401
 
 
 def compress_weights(model, **kwargs):

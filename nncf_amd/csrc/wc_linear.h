@@ -1,0 +1,295 @@
+// wc_linear.h -- shared by the kernels that multiply activations by compressed weights (wc_linear.hip, wc_gemm_nt.hip,
+// wc_experts.hip).
+//
+// The operator:  y[m, :] = act(x[m, :] . W^T + bias) + residual[m, :],  W [n, k] given as codes, scales and zero points.
+// W is the VALUE OF THE DECOMPRESSOR in the activations' type (wc_decompress.hip), bit for bit:
+//     integer modes, NF4:  RN_T(RN_fp16(d * s)),  d = code - zero point (or the code book's value in fp16), s fp16
+//     MXFP4:               RN_T(e2m1 * 2^(byte - 127))
+// so that a layer answers with the same weight whether it is decompressed first or multiplied as it is stored.  The sums,
+// the bias, the activation and the residual are fp32; the only rounding after the products is that of y.
+#pragma once
+#include "wc_common.h"
+
+namespace wc {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32v4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4, kActSwiglu = 5 };
+
+// ------------------------------------------------------------------------------------------ codes -> the weight's values
+// NF4's code book in fp16, as the decompressor holds it: one entry per code BYTE, the pair of its two nibbles
+constexpr int kNf4Pairs = 256;
+__device__ __constant__ const float kNf4Values[16] = {-1.0f, -0.6961928009986877f, -0.5250730514526367f, -0.39491748809814453f,
+                                                      -0.28444138169288635f, -0.18477343022823334f, -0.09105003625154495f, 0.0f,
+                                                      0.07958029955625534f, 0.16093020141124725f, 0.24611230194568634f,
+                                                      0.33791524171829224f, 0.44070982933044434f, 0.5626170039176941f,
+                                                      0.7229568362236023f, 1.0f};
+
+constexpr __host__ __device__ bool four_bit(int mode) { return mode >= NNCF_AMD_INT4_ASYM; }
+
+// what a group's scale and zero point become once: s2 the scale twice, z the zero points under the exponents that the codes
+// are given (see dequant8), e8 MXFP4's power of two
+template <int MODE>
+struct GroupPar {
+    h2 s2, z0, z1;
+    float e8;
+};
+
+template <int MODE>
+__device__ __forceinline__ GroupPar<MODE> group_par(const void* __restrict__ scale, const uint8_t* __restrict__ zp, int64_t g) {
+    GroupPar<MODE> p{};
+    if constexpr (MODE == NNCF_AMD_MXFP4) {
+        const uint32_t b = ((const uint8_t*)scale)[g];
+        p.e8 = __builtin_bit_cast(float, b ? b << 23 : 0x00400000u);  // byte 0: the subnormal 2^-127
+    } else {
+        const _Float16 s = __builtin_bit_cast(_Float16, ((const uint16_t*)scale)[g]);
+        p.s2 = h2{s, s};
+        if constexpr (MODE == NNCF_AMD_INT4_SYM || MODE == NNCF_AMD_INT4_ASYM) {
+            uint32_t z = 8;  // INT4_SYM: codes are stored with a +8 bias
+            if constexpr (MODE == NNCF_AMD_INT4_ASYM) z = (zp[g >> 1] >> (4 * (g & 1))) & 15u;
+            p.z0 = __builtin_bit_cast(h2, (0x6400u | z) * 0x00010001u);
+            p.z1 = __builtin_bit_cast(h2, (0x5400u | (z << 4)) * 0x00010001u);
+        } else if constexpr (MODE == NNCF_AMD_INT8_SYM || MODE == NNCF_AMD_INT8_ASYM) {
+            uint32_t z = 128;  // INT8_SYM: the sign bit is flipped, code + 128
+            if constexpr (MODE == NNCF_AMD_INT8_ASYM) z = zp[g];
+            p.z0 = __builtin_bit_cast(h2, (0x6400u | z) * 0x00010001u);
+        }
+    }
+    return p;
+}
+
+// two fp16 values -> two of the activations' type.  fp16 -> bf16 goes through fp32 (exact) and one rounding to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pair_of(_Float16 a, _Float16 b) {
+    if constexpr (DT == NNCF_AMD_F16) return __builtin_bit_cast(uint32_t, h2{a, b});
+    else return __builtin_bit_cast(uint32_t, b2{(__bf16)(float)a, (__bf16)(float)b});
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+    if constexpr (DT == NNCF_AMD_F16) return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
+    else return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+}
+
+// 8 consecutive weights of one group: p0 (4-bit modes: 8 nibbles, the lower first) or p0, p1 (8 bytes) -> four pairs.
+// A code enters as the fp16 number 1024 + c (its bits under the exponent 0x6400) or, where it sits four bits higher, as
+// 64 + c under 0x5400 (the units there are sixteenths), which saves the shift; the difference to 1024 + z or 64 + z is
+// exact and the packed product rounds once, as the decompressor does.
+template <int MODE, int DT>
+__device__ __forceinline__ u32v4 dequant8(uint32_t p0, uint32_t p1, const GroupPar<MODE>& g, const h2* lut) {
+    u32v4 r;
+    if constexpr (MODE == NNCF_AMD_MXFP4) {
+        if constexpr (DT == NNCF_AMD_BF16) {
+            r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, g.e8, 0));
+            r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, g.e8, 1));
+            r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, g.e8, 2));
+            r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(p0, g.e8, 3));
+        } else {
+            r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(p0, g.e8, 0));
+            r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(p0, g.e8, 1));
+            r.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(p0, g.e8, 2));
+            r.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(p0, g.e8, 3));
+        }
+    } else if constexpr (MODE == NNCF_AMD_NF4) {
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const h2 v = lut[(p0 >> (8 * k)) & 255u] * g.s2;
+            o[k] = pair_of<DT>(v.x, v.y);
+        }
+        r = u32v4{o[0], o[1], o[2], o[3]};
+    } else if constexpr (MODE == NNCF_AMD_INT4_SYM || MODE == NNCF_AMD_INT4_ASYM) {
+        const uint32_t q = p0 >> 8;
+        const h2 a = (__builtin_bit_cast(h2, (p0 & 0x000f000fu) | 0x64006400u) - g.z0) * g.s2;  // elements 0, 4
+        const h2 b = (__builtin_bit_cast(h2, (p0 & 0x00f000f0u) | 0x54005400u) - g.z1) * g.s2;  // 1, 5
+        const h2 c = (__builtin_bit_cast(h2, (q & 0x000f000fu) | 0x64006400u) - g.z0) * g.s2;   // 2, 6
+        const h2 d = (__builtin_bit_cast(h2, (q & 0x00f000f0u) | 0x54005400u) - g.z1) * g.s2;   // 3, 7
+        r = u32v4{pair_of<DT>(a.x, b.x), pair_of<DT>(c.x, d.x), pair_of<DT>(a.y, b.y), pair_of<DT>(c.y, d.y)};
+    } else {
+        uint32_t w[2] = {p0, p1};
+        if constexpr (MODE == NNCF_AMD_INT8_SYM) {
+            w[0] ^= 0x80808080u;
+            w[1] ^= 0x80808080u;
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t sel = (k & 1) ? 0x03070106u : 0x03050104u;  // bytes under the exponent byte 0x64
+            const h2 v = (__builtin_bit_cast(h2, __builtin_amdgcn_perm(w[k >> 1], 0x64006400u, sel)) - g.z0) * g.s2;
+            o[k] = pair_of<DT>(v.x, v.y);
+        }
+        r = u32v4{o[0], o[1], o[2], o[3]};
+    }
+    return r;
+}
+
+// one weight by its place (odd shapes)
+template <int MODE, int DT>
+__device__ __forceinline__ uint16_t dequant1(const uint8_t* __restrict__ codes, int64_t e, const GroupPar<MODE>& g, const h2* lut) {
+    uint32_t c;
+    if constexpr (four_bit(MODE)) c = (codes[e >> 1] >> (4 * (e & 1))) & 15u;
+    else c = codes[e];
+    return (uint16_t)dequant8<MODE, DT>(c, 0, g, lut).x;
+}
+
+template <int MODE>
+__device__ __forceinline__ void fill_nf4(h2* lut) {
+    if constexpr (MODE == NNCF_AMD_NF4) {
+        for (int i = threadIdx.x; i < kNf4Pairs; i += blockDim.x)
+            lut[i] = h2{(_Float16)kNf4Values[i & 15], (_Float16)kNf4Values[i >> 4]};
+        __syncthreads();
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------- activations
+// sigmoid as 1 / (1 + e^-z): e^-z = inf for z < -88 gives 0, the limit
+__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
+constexpr float kGeluC = 1.5957691216057308f;  // 2 * sqrt(2 / pi): tanh(u) written as 2 * sigmoid(2 u) - 1
+
+__device__ __forceinline__ float activate(int act, float z) {
+    switch (act) {
+        case kActRelu: return z > 0.0f ? z : (z == z ? 0.0f : z);
+        case kActGelu: return 0.5f * z * erfcf(-0.70710678118654752f * z);  // erfc keeps the small values of the left tail
+        case kActGeluTanh: return z * sigmoid_f(kGeluC * (z + 0.044715f * z * z * z));
+        case kActSilu: return z * sigmoid_f(z);
+        default: return z;
+    }
+}
+__device__ __forceinline__ float activate_grad(int act, float z) {
+    // far out every derivative has reached its limit; there z * z would overflow and meet a zero (a NaN passes)
+    z = z > 1e4f ? 1e4f : (z < -1e4f ? -1e4f : z);
+    switch (act) {
+        case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
+        case kActGelu: return 0.5f * erfcf(-0.70710678118654752f * z) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        case kActGeluTanh: {
+            const float s = sigmoid_f(kGeluC * (z + 0.044715f * z * z * z));
+            return s + z * s * (1.0f - s) * kGeluC * (1.0f + 0.134145f * z * z);
+        }
+        case kActSilu: {
+            const float s = sigmoid_f(z);
+            return s + z * s * (1.0f - s);
+        }
+        default: return 1.0f;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ float to_f32(uint16_t v) {
+    if constexpr (DT == NNCF_AMD_F16) return (float)__builtin_bit_cast(_Float16, v);
+    else return __builtin_bit_cast(float, (uint32_t)v << 16);
+}
+template <int DT>
+__device__ __forceinline__ uint16_t from_f32(float v) {
+    if constexpr (DT == NNCF_AMD_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
+    else return __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// --------------------------------------------------------------------------------------------------------------- problem
+// Where rows come from and how they are grouped.  offsets == nullptr: one weight, `rows` rows.  Else expert e owns the rows
+// [offsets[e], offsets[e + 1]) and the rows behind offsets[experts] get zeros.  slots != nullptr: row r reads x at
+// slots[r] / topk.  Both arrays are read with their values held to what the buffers have, so that a handle with other numbers
+// in it cannot reach memory that is not its own.
+struct RowMap {
+    const int32_t* offsets;
+    const int32_t* slots;
+    int32_t experts, topk;
+    int64_t rows, sources;  // rows of y; rows of x
+};
+__device__ __forceinline__ int64_t held(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
+__device__ __forceinline__ void expert_range(const RowMap& r, int e, int64_t& lo, int64_t& hi) {
+    if (!r.offsets) {
+        lo = 0, hi = r.rows;
+        return;
+    }
+    lo = held(r.offsets[e], 0, r.rows);
+    hi = held(r.offsets[e + 1], lo, r.rows);
+}
+__device__ __forceinline__ int64_t source_row(const RowMap& r, int64_t row) {
+    if (!r.slots) return row;
+    const int32_t s = r.slots[row];
+    return held((int64_t)((uint32_t)(s < 0 ? 0 : s) / (uint32_t)r.topk), 0, r.sources - 1);
+}
+
+struct Epilogue {
+    const void* bias;      // [n] or null
+    const void* residual;  // [rows, width] or null
+    void* y;               // [rows, width]
+    void* z;               // [rows, n] or null: the sums with their bias, for the gradient of the activation
+    int64_t ldr, ldy, n;   // n: rows of the weight; swiglu: gate rows first, width = n / 2
+    int act;
+    int y32;               // y is fp32 (gradients that are summed over rows afterwards)
+    int vec;               // 4 consecutive columns may be stored as 8 bytes (y, residual, z and their row strides allow it)
+};
+
+// up to four consecutive columns of one row; `up` only for swiglu (a: the gate's sums, b: the other half's)
+template <int DT>
+__device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t col, const float* a, const float* b) {
+    const int64_t width = e.act == kActSwiglu ? e.n / 2 : e.n;
+    if (col >= width) return;
+    const int cnt = width - col < 4 ? (int)(width - col) : 4;
+    float z[4], u[4], v[4];
+    const uint16_t* bias = (const uint16_t*)e.bias;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        z[i] = a[i];
+        u[i] = e.act == kActSwiglu ? b[i] : 0.0f;
+        if (bias && i < cnt) {
+            z[i] += to_f32<DT>(bias[col + i]);
+            if (e.act == kActSwiglu) u[i] += to_f32<DT>(bias[width + col + i]);
+        }
+        v[i] = e.act == kActSwiglu ? z[i] * sigmoid_f(z[i]) * u[i] : activate(e.act, z[i]);
+    }
+    uint16_t* y = (uint16_t*)e.y + row * e.ldy + col;
+    const uint16_t* res = e.residual ? (const uint16_t*)e.residual + row * e.ldr + col : nullptr;
+    uint16_t* zo = e.z ? (uint16_t*)e.z + row * e.n + col : nullptr;
+    if (e.y32) {
+        float* y32 = (float*)e.y + row * e.ldy + col;
+        if (e.vec && cnt == 4) *(f32x4*)y32 = f32x4{v[0], v[1], v[2], v[3]};
+        else
+            for (int i = 0; i < cnt; ++i) y32[i] = v[i];
+        return;
+    }
+    if (e.vec && cnt == 4) {
+        if (res) {
+            const u32v2 r = *(const u32v2*)res;
+            v[0] += to_f32<DT>((uint16_t)r.x), v[1] += to_f32<DT>((uint16_t)(r.x >> 16));
+            v[2] += to_f32<DT>((uint16_t)r.y), v[3] += to_f32<DT>((uint16_t)(r.y >> 16));
+        }
+        *(u32v2*)y = u32v2{pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3])};
+        if (zo) {
+            *(u32v2*)zo = u32v2{pair_of<DT>(z[0], z[1]), pair_of<DT>(z[2], z[3])};
+            if (e.act == kActSwiglu) *(u32v2*)(zo + width) = u32v2{pair_of<DT>(u[0], u[1]), pair_of<DT>(u[2], u[3])};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (i >= cnt) break;
+        if (res) v[i] += to_f32<DT>(res[i]);
+        y[i] = from_f32<DT>(v[i]);
+        if (zo) {
+            zo[i] = from_f32<DT>(z[i]);
+            if (e.act == kActSwiglu) zo[width + i] = from_f32<DT>(u[i]);
+        }
+    }
+}
+
+// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 32 and 16-byte rows, w [experts * n, k]
+struct DenseArgs {
+    const void* x;
+    const void* w;
+    int64_t ldx, k;
+    RowMap rows;
+    Epilogue ep;
+};
+// true where the tile kernels can address the operands (32-bit offsets from a tile's origin)
+bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gated, bool gathered);
+int dense_launch(int dtype, const DenseArgs& a, hipStream_t s);
+
+}  // namespace wc

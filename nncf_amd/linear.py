@@ -1,0 +1,250 @@
+"""Products with compressed weights: what a compressed layer computes, without its weight in between.
+
+The reference's Torch backend answers with a compressed layer in two steps, the decompressor module on every read of the weight
+(src/nncf/torch/quantization/layers.py:1303-1460) and a library product.  `compressed_linear` multiplies by the packed codes
+themselves, with bias, activation and residual in the product's epilogue and with the gradients that reach the activations
+(adapters that are trained beside frozen compressed weights).  The weight's values are bit for bit those of the decompressor,
+sums are fp32 and the result is rounded once.
+
+`fuse_compressed_linears` lets every `nn.Linear` of a compressed model answer this way.
+"""
+from __future__ import annotations
+
+import types
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+from torch.nn.utils import parametrize
+
+from nncf_amd import _lib
+from nncf_amd import decompressors as dcmp
+from nncf_amd.errors import InternalError
+
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "swiglu": 5}
+_SWIGLU = ACTIVATIONS["swiglu"]
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
+class PackedWeight(NamedTuple):
+    """A compressed weight as the kernels take it: [experts, n, k] codes with their scales and zero points."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    zero_point: Optional[torch.Tensor]
+    mode: int
+    experts: int
+    n: int
+    k: int
+    group_size: int
+
+
+def _mode_of(decompressor) -> str:
+    if isinstance(decompressor, dcmp._FourBit):
+        return decompressor._mode
+    if isinstance(decompressor, dcmp.INT8AsymmetricWeightsDecompressor):
+        return "int8_asym"
+    if isinstance(decompressor, dcmp.INT8SymmetricWeightsDecompressor):
+        return "int8_sym"
+    raise InternalError(f"{type(decompressor).__name__} is not a decompressor of this package")
+
+
+def weight_dtype_of(decompressor) -> torch.dtype:
+    """Type of the weight that `decompressor` returns."""
+    if decompressor.result_dtype is not None:
+        return decompressor.result_dtype
+    return torch.float16
+
+
+def packed_weight(packed: torch.Tensor, decompressor, x: torch.Tensor, ndim: int, what: str) -> PackedWeight:
+    """`packed` and its decompressor as the kernels take them; ndim: 2 for [n, k], 3 for [experts, n, k]."""
+    mode = _mode_of(decompressor)
+    if x.dtype not in _DTYPES:
+        raise InternalError(f"{what}: activations are float16 or bfloat16, got {x.dtype}")
+    if weight_dtype_of(decompressor) != x.dtype:
+        raise InternalError(f"{what}: activations are {x.dtype}, the decompressed weight is {weight_dtype_of(decompressor)}")
+    scale = decompressor._scale
+    four = isinstance(decompressor, dcmp._FourBit)
+    if four:
+        grouped = tuple(decompressor.compressed_weight_shape)
+        shape = grouped if decompressor.result_shape is None else tuple(decompressor.result_shape)
+    else:
+        shape = grouped = tuple(packed.shape)
+    if len(shape) != ndim or 0 in shape:
+        raise InternalError(f"{what}: the weight is {ndim}-dimensional and not empty, got shape {shape}")
+    n_groups, group_size = dcmp._groups(grouped, scale)
+    experts, (n, k) = (1 if ndim == 2 else shape[0]), shape[-2:]
+    if n_groups * group_size != experts * n * k or k % group_size:
+        raise InternalError(f"{what}: groups of {group_size} do not divide rows of {k} (weight {shape}, scale {tuple(scale.shape)})")
+    codes = packed.detach()
+    if codes.dtype != (torch.int8 if mode == "int8_sym" else torch.uint8):
+        raise InternalError(f"{what}: packed codes of type {codes.dtype} for mode {mode}")
+    if codes.numel() != (experts * n * k // 2 if four else experts * n * k):
+        raise InternalError(f"{what}: {codes.numel()} bytes of codes for a weight of shape {shape}, mode {mode}")
+    if scale.dtype != (torch.uint8 if mode == "mxfp4" else torch.float16):
+        raise InternalError(f"{what}: scales of type {scale.dtype} for mode {mode}")
+    zp = getattr(decompressor, "_zero_point", None)
+    for t in (codes, scale, zp):
+        if t is not None and t.device != x.device:
+            raise InternalError(f"{what}: the weight is on {t.device}, the activations on {x.device}")
+    if zp is not None:
+        if zp.dtype != torch.uint8 or zp.numel() != ((n_groups + 1) // 2 if four else n_groups):
+            raise InternalError(f"{what}: {zp.numel()} bytes of zero points ({zp.dtype}) for {n_groups} groups, mode {mode}")
+        zp = zp.contiguous()
+    return PackedWeight(codes.contiguous(), scale.contiguous(), zp, _lib.MODE_ID[mode], experts, n, k, group_size)
+
+
+def activation_of(activation: Optional[str], n: int, what: str) -> Tuple[int, int]:
+    """(number of the activation, columns of the result)."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{what}: unknown activation {activation!r}, expected one of {list(ACTIVATIONS)}")
+    act = ACTIVATIONS[activation]
+    if act != _SWIGLU:
+        return act, n
+    if n % 2:
+        raise ValueError(f"{what}: swiglu needs an even number of weight rows, got {n}")
+    return act, n // 2
+
+
+def rows_of(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
+    """`t` [..., width] as rows of consecutive elements and their distance (copied where its strides do not allow it)."""
+    t = t.reshape(-1, width)
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else width
+
+
+def workspace_of(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def activation_grad(dy: torch.Tensor, z: Optional[torch.Tensor], n: int, act: int, dtype: torch.dtype, want_dz: bool, want_dbias: bool):
+    """(dz, its row stride, dbias) of the epilogue: dz = dy * act'(z), padded to whole steps of the product that follows."""
+    width = n // 2 if act == _SWIGLU else n
+    dy, ldd = rows_of(dy, width)
+    m = dy.shape[0]
+    if act == 0 and not want_dbias:
+        return dy, ldd, None
+    L = _lib.lib()
+    copies = want_dz and act != 0  # without an activation dz is dy
+    ldz = (n + 31) // 32 * 32
+    dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
+    dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
+    ws = workspace_of(L.nncf_amd_activation_grad_workspace(m, n) if want_dbias else 0, dy.device)
+    _lib.check(L.nncf_amd_activation_grad(_lib.ptr(dy), _DTYPES[dtype], ldd, _lib.ptr(z), m, n, act, _lib.ptr(dz), ldz, _lib.ptr(dbias),
+                                          _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(dy)))
+    return (dz, ldz, dbias) if copies else (dy, ldd, dbias)
+
+
+def grad_input(dz: torch.Tensor, ldz: int, w: PackedWeight, offsets: Optional[torch.Tensor], dtype: torch.dtype,
+               fp32: bool = False) -> torch.Tensor:
+    L = _lib.lib()
+    m = dz.shape[0]
+    dx = torch.empty((m, w.k), dtype=torch.float32 if fp32 else dtype, device=dz.device)
+    ws = workspace_of(L.nncf_amd_linear_grad_input_workspace(_lib.ptr(dz), ldz, m, w.n, w.k, w.experts), dz.device)
+    _lib.check(L.nncf_amd_linear_grad_input(_lib.ptr(dz), _DTYPES[dtype], ldz, _lib.ptr(offsets), w.experts, m, w.n, w.k, _lib.ptr(w.codes),
+                                            w.mode, w.group_size, _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(dx), w.k, int(fp32),
+                                            _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(dz)))
+    return dx
+
+
+def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_z: bool):
+    """(y [m, width], z [m, n] or None) of rows x [..., k]."""
+    rows, ldx = rows_of(x, w.k)
+    m = rows.shape[0]
+    y = torch.empty((m, width), dtype=x.dtype, device=x.device)
+    z = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if want_z else None
+    res, ldr = (None, 0) if residual is None else rows_of(residual, width)
+    L = _lib.lib()
+    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(_lib.ptr(rows), ldx, m, w.n, w.k, w.mode, w.group_size), x.device)
+    _lib.check(L.nncf_amd_compressed_linear(_lib.ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
+                                            _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(bias), act, _lib.ptr(res), ldr,
+                                            _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws), 0 if ws is None else ws.numel(),
+                                            _lib.stream_of(x)))
+    return y, z
+
+
+class _CompressedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, bias, residual, w, act, width):
+        with torch.cuda.device(x.device):
+            y, z = _forward(x, w, bias, act, width, residual, act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]))
+        ctx.save_for_backward(z, w.codes, w.scale, w.zero_point)
+        ctx.weight, ctx.act, ctx.shape, ctx.dtype = w[3:], act, x.shape, x.dtype
+        return y.reshape(x.shape[:-1] + (width,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        z, codes, scale, zp = ctx.saved_tensors
+        w = PackedWeight(codes, scale, zp, *ctx.weight)
+        need_x, need_bias, need_residual = ctx.needs_input_grad[:3]
+        dx = dbias = None
+        if need_x or need_bias:
+            with torch.cuda.device(dy.device):
+                dz, ldz, dbias = activation_grad(dy, z, w.n, ctx.act, ctx.dtype, need_x, need_bias)
+                if need_x:
+                    dx = grad_input(dz, ldz, w, None, ctx.dtype).reshape(ctx.shape)
+        return dx, dbias, dy if need_residual else None, None, None, None
+
+
+def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias: Optional[torch.Tensor] = None,
+                      activation: Optional[str] = None, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x W^T + bias) + residual with W = decompressor(packed), which is never written to memory in the layer's place.
+
+    x            [..., in_features], float16 or bfloat16, any strides; the type of the decompressed weight
+    packed       the packed codes of a [out_features, in_features] weight, with their decompressor (`nncf_amd.decompressors`)
+    bias         [out_features] in x's type
+    activation   None, "relu", "gelu", "gelu_tanh", "silu", or "swiglu": the first half of W's rows is the gate, the result
+                 silu(gate) * up has out_features / 2 columns
+    residual     the result's shape and type
+
+    Differentiable in x, bias and residual (not twice); the weight is frozen.  With an activation the backward pass keeps the
+    sums in x's type."""
+    what = "compressed_linear"
+    _lib.require_gpu(x, what)
+    w = packed_weight(packed, decompressor, x, 2, what)
+    act, width = activation_of(activation, w.n, what)
+    if x.ndim < 1 or x.shape[-1] != w.k:
+        raise InternalError(f"{what}: x of shape {tuple(x.shape)} for a weight with {w.k} input features")
+    if bias is not None:
+        if tuple(bias.shape) != (w.n,) or bias.dtype != x.dtype or bias.device != x.device:
+            raise InternalError(f"{what}: bias {tuple(bias.shape)} {bias.dtype} on {bias.device}, expected ({w.n},) {x.dtype} on {x.device}")
+    if residual is not None:
+        if tuple(residual.shape) != tuple(x.shape[:-1]) + (width,) or residual.dtype != x.dtype or residual.device != x.device:
+            raise InternalError(f"{what}: residual {tuple(residual.shape)} {residual.dtype} on {residual.device}, expected "
+                                f"{tuple(x.shape[:-1]) + (width,)} {x.dtype} on {x.device}")
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+        return _CompressedLinear.apply(x, bias, residual, w, act, width)
+    with torch.cuda.device(x.device):
+        y, _ = _forward(x, w, bias, act, width, residual, False)
+    return y.reshape(x.shape[:-1] + (width,))
+
+
+# ------------------------------------------------------------------------------------------------------------- models
+def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:
+    plist = self.parametrizations.weight
+    if not x.is_cuda or torch.is_autocast_enabled("cuda") or x.dtype != weight_dtype_of(plist[0]):
+        return nn.Linear.forward(self, x)  # a library product in another type, as before
+    return compressed_linear(x, plist.original, plist[0], bias=self.bias)
+
+
+def fuse_compressed_linears(model: nn.Module) -> int:
+    """Lets every `nn.Linear` of a compressed model (`nncf_amd.compress_weights`, `load_compressed`) whose weight is float16 or
+    bfloat16 answer through `compressed_linear` instead of decompressing its weight and calling a library product.  In place;
+    parameters, state_dict keys and `save_compressed` stay as they are, results differ by the sums' order only.  Returns how
+    many modules now do."""
+    count = 0
+    for mod in model.modules():
+        if not isinstance(mod, nn.Linear) or not parametrize.is_parametrized(mod, "weight"):
+            continue
+        plist = mod.parametrizations.weight
+        if len(plist) != 1 or not isinstance(plist[0], dcmp.BaseWeightsDecompressor) or weight_dtype_of(plist[0]) not in _DTYPES:
+            continue
+        if mod.bias is not None and mod.bias.dtype != weight_dtype_of(plist[0]):
+            continue
+        mod.forward = types.MethodType(_fused_forward, mod)
+        count += 1
+    return count
