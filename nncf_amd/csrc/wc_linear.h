@@ -42,27 +42,30 @@ struct GroupPar {
     float e8;
 };
 
+// from a group's raw scale (fp16 bits or E8M0 byte) and zero point
 template <int MODE>
-__device__ __forceinline__ GroupPar<MODE> group_par(const void* __restrict__ scale, const uint8_t* __restrict__ zp, int64_t g) {
+__device__ __forceinline__ GroupPar<MODE> par_of(uint32_t scale, uint32_t zero) {
     GroupPar<MODE> p{};
     if constexpr (MODE == NNCF_AMD_MXFP4) {
-        const uint32_t b = ((const uint8_t*)scale)[g];
-        p.e8 = __builtin_bit_cast(float, b ? b << 23 : 0x00400000u);  // byte 0: the subnormal 2^-127
+        p.e8 = __builtin_bit_cast(float, scale ? scale << 23 : 0x00400000u);  // byte 0: the subnormal 2^-127
     } else {
-        const _Float16 s = __builtin_bit_cast(_Float16, ((const uint16_t*)scale)[g]);
+        const _Float16 s = __builtin_bit_cast(_Float16, (uint16_t)scale);
         p.s2 = h2{s, s};
-        if constexpr (MODE == NNCF_AMD_INT4_SYM || MODE == NNCF_AMD_INT4_ASYM) {
-            uint32_t z = 8;  // INT4_SYM: codes are stored with a +8 bias
-            if constexpr (MODE == NNCF_AMD_INT4_ASYM) z = (zp[g >> 1] >> (4 * (g & 1))) & 15u;
-            p.z0 = __builtin_bit_cast(h2, (0x6400u | z) * 0x00010001u);
-            p.z1 = __builtin_bit_cast(h2, (0x5400u | (z << 4)) * 0x00010001u);
-        } else if constexpr (MODE == NNCF_AMD_INT8_SYM || MODE == NNCF_AMD_INT8_ASYM) {
-            uint32_t z = 128;  // INT8_SYM: the sign bit is flipped, code + 128
-            if constexpr (MODE == NNCF_AMD_INT8_ASYM) z = zp[g];
-            p.z0 = __builtin_bit_cast(h2, (0x6400u | z) * 0x00010001u);
-        }
+        if constexpr (MODE == NNCF_AMD_INT4_SYM) zero = 8;    // codes are stored with a +8 bias
+        if constexpr (MODE == NNCF_AMD_INT8_SYM) zero = 128;  // dequant8 flips the sign bit: code + 128
+        if constexpr (MODE != NNCF_AMD_NF4) p.z0 = __builtin_bit_cast(h2, (0x6400u | zero) * 0x00010001u);
+        if constexpr (MODE == NNCF_AMD_INT4_SYM || MODE == NNCF_AMD_INT4_ASYM)
+            p.z1 = __builtin_bit_cast(h2, (0x5400u | (zero << 4)) * 0x00010001u);
     }
     return p;
+}
+template <int MODE>
+__device__ __forceinline__ GroupPar<MODE> group_par(const void* __restrict__ scale, const uint8_t* __restrict__ zp, int64_t g) {
+    uint32_t z = 0;
+    if constexpr (MODE == NNCF_AMD_INT4_ASYM) z = (zp[g >> 1] >> (4 * (g & 1))) & 15u;
+    if constexpr (MODE == NNCF_AMD_INT8_ASYM) z = zp[g];
+    if constexpr (MODE == NNCF_AMD_MXFP4) return par_of<MODE>(((const uint8_t*)scale)[g], z);
+    else return par_of<MODE>(((const uint16_t*)scale)[g], z);
 }
 
 // two fp16 values -> two of the activations' type.  fp16 -> bf16 goes through fp32 (exact) and one rounding to nearest even.
@@ -105,11 +108,14 @@ __device__ __forceinline__ u32v4 dequant8(uint32_t p0, uint32_t p1, const GroupP
         }
         r = u32v4{o[0], o[1], o[2], o[3]};
     } else if constexpr (MODE == NNCF_AMD_INT4_SYM || MODE == NNCF_AMD_INT4_ASYM) {
+        // masks in scalar and exponents in vector registers: one v_and_or_b32 each (as literals they take two instructions)
+        uint32_t m0 = 0x000f000fu, m1 = 0x00f000f0u, e0 = 0x64006400u, e1 = 0x54005400u;
+        asm("" : "+s"(m0), "+s"(m1), "+v"(e0), "+v"(e1));
         const uint32_t q = p0 >> 8;
-        const h2 a = (__builtin_bit_cast(h2, (p0 & 0x000f000fu) | 0x64006400u) - g.z0) * g.s2;  // elements 0, 4
-        const h2 b = (__builtin_bit_cast(h2, (p0 & 0x00f000f0u) | 0x54005400u) - g.z1) * g.s2;  // 1, 5
-        const h2 c = (__builtin_bit_cast(h2, (q & 0x000f000fu) | 0x64006400u) - g.z0) * g.s2;   // 2, 6
-        const h2 d = (__builtin_bit_cast(h2, (q & 0x00f000f0u) | 0x54005400u) - g.z1) * g.s2;   // 3, 7
+        const h2 a = (__builtin_bit_cast(h2, (p0 & m0) | e0) - g.z0) * g.s2;  // elements 0, 4
+        const h2 b = (__builtin_bit_cast(h2, (p0 & m1) | e1) - g.z1) * g.s2;  // 1, 5
+        const h2 c = (__builtin_bit_cast(h2, (q & m0) | e0) - g.z0) * g.s2;   // 2, 6
+        const h2 d = (__builtin_bit_cast(h2, (q & m1) | e1) - g.z1) * g.s2;   // 3, 7
         r = u32v4{pair_of<DT>(a.x, b.x), pair_of<DT>(c.x, d.x), pair_of<DT>(a.y, b.y), pair_of<DT>(c.y, d.y)};
     } else {
         uint32_t w[2] = {p0, p1};
@@ -291,5 +297,19 @@ struct DenseArgs {
 // true where the tile kernels can address the operands (32-bit offsets from a tile's origin)
 bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gated, bool gathered);
 int dense_launch(int dtype, const DenseArgs& a, hipStream_t s);
+
+// the product for few rows per group, from the codes (wc_linear_few.hip): groups and rows of whole 32 k, 16-byte rows
+struct FewArgs {
+    const void* x;
+    int64_t ldx;
+    const uint8_t* codes;
+    const void* scale;
+    const uint8_t* zp;
+    uint32_t k, groups, magic;  // groups per row; magic: ceil(2^32 / (group size / 32)), 0 for groups of 32
+    RowMap rows;
+    Epilogue ep;
+};
+bool few_fits(int mode, int64_t k, int64_t gs, const void* codes);
+int few_launch(int dtype, int mode, const FewArgs& a, hipStream_t s);
 
 }  // namespace wc

@@ -292,21 +292,27 @@ int check_pointers(const char* what, const Weight& w) {
     return NNCF_AMD_OK;
 }
 
-// What a call's workspace holds, one behind the other: the decompressed weight, the packed rows of x.
+// What a call's workspace holds, one behind the other: the decompressed weight, the packed rows of x; and whether the product
+// runs on the codes themselves.
 struct Need {
     size_t weight, pack;
+    bool few;
     size_t total() const { return weight + pack; }
 };
+// rows per group up to which the codes are multiplied as they are
+constexpr int64_t kFewRows = 16;
 bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gathered) {
     return k % 32 || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
 }
 Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows) {
-    Need d{(size_t)(w.experts * w.n * round32(w.k)) * 2, 0};
-    if (must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round32(w.k)) * 2;
+    Need d{(size_t)(w.experts * w.n * round32(w.k)) * 2, 0, false};
+    d.few = rows <= kFewRows * w.experts && few_fits(w.mode, w.k, w.gs, w.codes);
+    if (d.few) d.weight = 0;
+    if (d.few ? ldx % 8 || ((uintptr_t)x & 15) : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round32(w.k)) * 2;
     return d;
 }
 Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
-    Need d{(size_t)(w.experts * w.k * round32(w.n)) * 2, 0};
+    Need d{(size_t)(w.experts * w.k * round32(w.n)) * 2, 0, false};
     if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * round32(w.n)) * 2;
     return d;
 }
@@ -318,17 +324,22 @@ int vec_of(const Epilogue& e) {
     return (bits & 7) == 0 && e.ldy % 4 == 0 && (!e.residual || e.ldr % 4 == 0) && (!e.z || width % 4 == 0);
 }
 
+int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* pack, hipStream_t s) {
+    const int64_t kp = round32(k);
+    if (rows.rows > 0x7fffffff) {
+        set_error("linear: too many rows");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)rows.rows), dim3(256), 0, s, (const uint16_t*)x, ldx, k, kp, pack, rows);
+    x = pack, ldx = kp, rows.slots = nullptr, rows.sources = rows.rows;
+    return launch_status("linear: rows");
+}
+
 int run_dense(int dtype, const void* x, int64_t ldx, int64_t k, const void* w, RowMap rows, Epilogue ep, uint16_t* pack, hipStream_t s) {
     const int64_t kp = round32(k);
     if (must_pack(x, ldx, k, rows.sources, rows.slots != nullptr)) {
-        if (rows.rows > 0x7fffffff) {
-            set_error("linear: too many rows");
-            return NNCF_AMD_ERR_UNSUPPORTED;
-        }
-        hipLaunchKernelGGL(k_pack_rows, dim3((unsigned)rows.rows), dim3(256), 0, s, (const uint16_t*)x, ldx, k, kp, pack, rows);
-        const int st = launch_status("linear: rows");
+        const int st = pack_rows(x, ldx, k, rows, pack, s);
         if (st != NNCF_AMD_OK) return st;
-        x = pack, ldx = kp, rows.slots = nullptr, rows.sources = rows.rows;
     }
     if (!dense_reaches(ep.n, kp, ldx, rows.sources, ep.act == kActSwiglu, rows.slots != nullptr)) {
         set_error("linear: operands beyond the kernels' range (n=%lld k=%lld)", (long long)ep.n, (long long)k);
@@ -360,6 +371,18 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
     if (need.total() && (!ws || ws_bytes < need.total() || ((uintptr_t)ws & 15))) {
         set_error("%s: workspace of %zu bytes, aligned to 16, needed", what, need.total());
         return NNCF_AMD_ERR_WORKSPACE;
+    }
+    if (need.few) {
+        RowMap map = rows;
+        if (need.pack) {
+            st = pack_rows(x, ldx, w.k, map, (uint16_t*)ws, s);
+            if (st != NNCF_AMD_OK) return st;
+        }
+        const uint32_t g32 = (uint32_t)(w.gs / 32);
+        const uint32_t magic = g32 == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + g32 - 1) / g32);
+        Epilogue e = ep;
+        e.vec = vec_of(e);
+        return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, (uint32_t)(w.k / w.gs), magic, map, e}, s);
     }
     uint16_t* dense = (uint16_t*)ws;
     st = dtype == NNCF_AMD_BF16 ? dequant_rows<NNCF_AMD_BF16>(w, rows, dense, s) : dequant_rows<NNCF_AMD_F16>(w, rows, dense, s);
@@ -403,11 +426,11 @@ int check_groups(const char* what, const int32_t* offsets, const int32_t* slots,
 
 }  // namespace wc
 
-extern "C" size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, int mode,
-                                                       int64_t group_size) {
+extern "C" size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes,
+                                                       int mode, int64_t group_size) {
     using namespace wc;
     if (m < 1 || n < 1 || k < 1) return 0;
-    const Weight w{nullptr, nullptr, nullptr, mode, n, k, group_size, 1};
+    const Weight w{(const uint8_t*)codes, nullptr, nullptr, mode, n, k, group_size == -1 ? k : group_size, 1};
     return forward_need(w, x, ldx, m, false, m).total();
 }
 
@@ -430,10 +453,10 @@ extern "C" int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx,
 }
 
 extern "C" size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, int64_t sources, int gathered, int64_t rows, int64_t n,
-                                                   int64_t k, int mode, int64_t group_size, int64_t experts) {
+                                                   int64_t k, const void* codes, int mode, int64_t group_size, int64_t experts) {
     using namespace wc;
     if (rows < 1 || n < 1 || k < 1 || experts < 1) return 0;
-    const Weight w{nullptr, nullptr, nullptr, mode, n, k, group_size, experts};
+    const Weight w{(const uint8_t*)codes, nullptr, nullptr, mode, n, k, group_size == -1 ? k : group_size, experts};
     return forward_need(w, x, ldx, sources, gathered != 0, rows).total();
 }
 

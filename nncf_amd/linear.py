@@ -156,7 +156,8 @@ def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_z: b
     z = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if want_z else None
     res, ldr = (None, 0) if residual is None else rows_of(residual, width)
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(_lib.ptr(rows), ldx, m, w.n, w.k, w.mode, w.group_size), x.device)
+    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(_lib.ptr(rows), ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode,
+                                                             w.group_size), x.device)
     _lib.check(L.nncf_amd_compressed_linear(_lib.ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
                                             _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(bias), act, _lib.ptr(res), ldr,
                                             _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws), 0 if ws is None else ws.numel(),
