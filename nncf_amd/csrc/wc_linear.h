@@ -249,6 +249,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
             z[i] += to_f32<DT>(bias[col + i]);
             if (e.act == kActSwiglu) u[i] += to_f32<DT>(bias[width + col + i]);
         }
+        __builtin_amdgcn_sched_barrier(0);  // one after the other: side by side their exponentials need the most registers
         v[i] = e.act == kActSwiglu ? z[i] * sigmoid_f(z[i]) * u[i] : activate(e.act, z[i]);
     }
     uint16_t* y = (uint16_t*)e.y + row * e.ldy + col;
@@ -298,18 +299,19 @@ struct DenseArgs {
 bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gated, bool gathered);
 int dense_launch(int dtype, const DenseArgs& a, hipStream_t s);
 
-// the product for few rows per group, from the codes (wc_linear_few.hip): groups and rows of whole 32 k, 16-byte rows
+// the product for few rows per group, from the codes (wc_linear_few.hip): rows of whole 32 k, groups of 32, of whole 64 or the row, 16-byte rows of x
 struct FewArgs {
     const void* x;
     int64_t ldx;
     const uint8_t* codes;
     const void* scale;
     const uint8_t* zp;
-    uint32_t k, groups, magic;  // groups per row; magic: ceil(2^32 / (group size / 32)), 0 for groups of 32
+    uint32_t k, groups, magic;  // groups per row; magic: ceil(2^32 / (group size / 16))
+    uint32_t scales8;           // ceil(2^32 / (groups / 8)) where rows have whole eight groups, aligned in memory; else 0
     RowMap rows;
     Epilogue ep;
 };
-bool few_fits(int mode, int64_t k, int64_t gs, const void* codes);
+bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t sources, int64_t ldx);
 int few_launch(int dtype, int mode, const FewArgs& a, hipStream_t s);
 
 }  // namespace wc

@@ -306,9 +306,10 @@ bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gath
 }
 Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows) {
     Need d{(size_t)(w.experts * w.n * round32(w.k)) * 2, 0, false};
-    d.few = rows <= kFewRows * w.experts && few_fits(w.mode, w.k, w.gs, w.codes);
+    const bool copy = ldx % 8 || ((uintptr_t)x & 15);
+    d.few = rows <= kFewRows * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? round32(w.k) : ldx);
     if (d.few) d.weight = 0;
-    if (d.few ? ldx % 8 || ((uintptr_t)x & 15) : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round32(w.k)) * 2;
+    if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round32(w.k)) * 2;
     return d;
 }
 Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
@@ -378,11 +379,15 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
             st = pack_rows(x, ldx, w.k, map, (uint16_t*)ws, s);
             if (st != NNCF_AMD_OK) return st;
         }
-        const uint32_t g32 = (uint32_t)(w.gs / 32);
-        const uint32_t magic = g32 == 1 ? 0 : (uint32_t)((((uint64_t)1 << 32) + g32 - 1) / g32);
+        const uint32_t g16 = (uint32_t)(w.gs / 16);  // at least 2: groups of whole 32
+        const uint32_t magic = (uint32_t)((((uint64_t)1 << 32) + g16 - 1) / g16);
+        const uint32_t groups = (uint32_t)(w.k / w.gs);
+        // (more than eight groups, so that the multiplier fits; their number times 16 rows of 8 strips stays far below 2^32)
+        const bool eights = groups % 8 == 0 && groups > 8 && (((uintptr_t)w.scale | (uintptr_t)w.zp) & 15) == 0;
+        const uint32_t scales8 = eights ? (uint32_t)((((uint64_t)1 << 32) + groups / 8 - 1) / (groups / 8)) : 0;
         Epilogue e = ep;
         e.vec = vec_of(e);
-        return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, (uint32_t)(w.k / w.gs), magic, map, e}, s);
+        return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, groups, magic, scales8, map, e}, s);
     }
     uint16_t* dense = (uint16_t*)ws;
     st = dtype == NNCF_AMD_BF16 ? dequant_rows<NNCF_AMD_BF16>(w, rows, dense, s) : dequant_rows<NNCF_AMD_F16>(w, rows, dense, s);

@@ -1,11 +1,19 @@
 // wc_linear_few.hip -- the product with a compressed weight for few rows of x (a token per sequence): up to 16 of them, or as many
-// per expert, at a time.  Bound by the bytes of the codes (0.5-1 per weight), which are read once and dequantised in registers.
+// per expert, at a time.  The codes (0.5-1 byte per weight) are read once and dequantised in registers.
 //
-// A block owns 16 * R rows of W; its waves take consecutive parts of k and add their sums through LDS.  A lane holds row
-// (lane & 15) and 32 consecutive k of a step of 128 (the four quarters of the wave side by side): one 16-byte load of 4-bit
-// codes, all of one group.  That is the A operand of four v_mfma_f32_16x16x32 whose B operand is the same 32 k of x's row
-// (lane & 15): the order of k inside a step is free as long as both operands share it.  The codes, scales and x of the next
-// step are requested before the current one is used.
+// A block owns WN strips of 16 rows of W and cuts k into WK parts, one wave for each pair (up to 16), all in step; one block per
+// compute unit where the strips allow it, so that there is one start and one end.  A wave's step is 256 k (128 with 8-bit
+// codes) of its strip: 16 rows x 128 bytes, whole lines, eight lanes a row (a load straight into the operand's layout, 16 rows
+// x 64 bytes, reaches 3.3 TB/s on a 28672 x 8192 weight, this one 5.0), turned round in 2 KiB of LDS of the wave's own; the
+// rows' 16-byte chunks are permuted (c ^ (row >> 1)) so that both sides touch all banks.  From there a lane takes 8 bytes of row
+// (lane & 15) at a time: the A operand of one (8-bit codes) or two v_mfma_f32_16x16x32.  The codes of the next two steps are
+// on their way meanwhile.
+// x, four to eight times the codes' bytes if every strip read it by itself and in the operand's scattered order, comes to LDS in
+// whole rows, once for the waves that share a part of k, a step ahead (two buffers, one barrier a step).  The strips' scales
+// and zero points, one run of memory, come to LDS at the start: a scattered load of two bytes a lane takes the load unit about
+// as many cycles as it has lanes.
+#include <type_traits>
+
 #include "wc_linear.h"
 
 namespace wc {
@@ -13,7 +21,8 @@ namespace wc {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 16;
+constexpr int kFewLdsBytes = 160 * 1024 - 1024;  // less the NF4 table
 
 template <int DT>
 __device__ __forceinline__ f32x4 mfma16(const u32v4& a, const u32v4& b, f32x4 c) {
@@ -23,170 +32,335 @@ __device__ __forceinline__ f32x4 mfma16(const u32v4& a, const u32v4& b, f32x4 c)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-template <int MODE, int R>
-struct FewStep {
-    u32v4 codes[R][four_bit(MODE) ? 1 : 2];
-    uint32_t scale[R], zero[R];
-    u32v4 x[4];
+// A block's shape and its LDS: codes [wave][2 KiB] (at the end the waves' sums), x [buffer][part][row][512 bytes (8-bit codes:
+// 256)], scales [strip][group][16 rows], zero points.
+struct FewShape {
+    int wn, wk, rows, buffers;    // rows of x at a time
+    int steps, per_wk;            // steps of a wave; ceil(2^16 / wk)
+    int pitch;                    // groups of a row, and one place more
+    int scale_bytes, zero_bytes;  // per group; zero_bytes 0: none
+    int x_bytes;                  // of a row and step
+    __host__ __device__ int waves() const { return wn * wk; }
+    __host__ __device__ int x() const { return waves() * 2048; }
+    __host__ __device__ int scales() const { return x() + buffers * wk * rows * x_bytes; }
+    __host__ __device__ int zeros() const { return scales() + (wn * 16 * pitch * scale_bytes + 15) / 16 * 16; }
+    __host__ __device__ int total() const { return zeros() + wn * 16 * pitch * zero_bytes; }
 };
 
-template <int MODE, int DT, int R>
-__global__ __launch_bounds__(64 * kFewWaves, 4) void k_few_rows(FewArgs a) {
+// XI: loads of two rows of x (8-bit codes: four) that a wave makes per step; 8 of them need the registers of 16 waves for 8
+template <int MODE, int DT, int XI>
+__global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_rows(FewArgs a, FewShape sh) {
+    constexpr int MF = four_bit(MODE) ? 2 : 1;           // matrix instructions per 8 bytes of codes
+    constexpr uint32_t KS = four_bit(MODE) ? 256 : 128;  // k of a step
+    constexpr int XROWS = 1024 / (2 * KS);               // rows of x per load, 16 bytes a lane
+    constexpr bool ASYM = MODE == NNCF_AMD_INT4_ASYM || MODE == NNCF_AMD_INT8_ASYM;
+    using scale_t = typename std::conditional<MODE == NNCF_AMD_MXFP4, uint8_t, uint16_t>::type;
     __shared__ h2 lut[MODE == NNCF_AMD_NF4 ? kNf4Pairs : 1];
-    __shared__ f32x4 part[kFewWaves][R][64];
+    extern __shared__ __align__(16) char dyn[];
     fill_nf4<MODE>(lut);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r16 = lane & 15, kq = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wave * sh.per_wk >> 16, wk = wave - wn * sh.wk;
+    char* mine = dyn + wave * 2048;
+    char* xbuf = dyn + sh.x();
+    scale_t* scales = (scale_t*)(dyn + sh.scales());
+    uint8_t* zeros = (uint8_t*)(dyn + sh.zeros());
     const int expert = blockIdx.y;
     const bool gated = a.ep.act == kActSwiglu;
     const int64_t n = a.ep.n, width = gated ? n / 2 : n;
-    const int tiles = gated ? R / 2 : R;  // tiles of 16 columns of y
-    const int64_t col0 = (int64_t)blockIdx.x * 16 * tiles;
+    // strip w of the block: 16 columns of y; with a gate the even ones are the gate's rows, the odd ones the other half's
+    auto column_of = [&](int w) { return gated ? ((int64_t)blockIdx.x * (sh.wn / 2) + (w >> 1)) * 16 : ((int64_t)blockIdx.x * sh.wn + w) * 16; };
     int64_t lo, hi;
     if (a.rows.offsets && expert == 0) {  // rows behind the last group are zero
         expert_range(a.rows, a.rows.experts - 1, lo, hi);
-        for (int64_t r = hi + wave; r < a.rows.rows; r += kFewWaves)
-            if (lane < 16 * tiles && col0 + lane < width) {
-                ((uint16_t*)a.ep.y)[r * a.ep.ldy + col0 + lane] = 0;
+        const int64_t c0 = column_of(0), c1 = c0 + (gated ? sh.wn / 2 : sh.wn) * 16 < width ? c0 + (gated ? sh.wn / 2 : sh.wn) * 16 : width;
+        for (int64_t r = hi + wave; r < a.rows.rows; r += sh.waves())
+            for (int64_t c = c0 + lane; c < c1; c += 64) {
+                ((uint16_t*)a.ep.y)[r * a.ep.ldy + c] = 0;
                 if (a.ep.z) {
-                    ((uint16_t*)a.ep.z)[r * n + col0 + lane] = 0;
-                    if (gated) ((uint16_t*)a.ep.z)[r * n + width + col0 + lane] = 0;
+                    ((uint16_t*)a.ep.z)[r * n + c] = 0;
+                    if (gated) ((uint16_t*)a.ep.z)[r * n + width + c] = 0;
                 }
             }
     }
     expert_range(a.rows, expert, lo, hi);
     if (lo >= hi) return;
 
-    const uint32_t k = a.k, steps = (k + 127) / 128, per_wave = (steps + kFewWaves - 1) / kFewWaves;
-    const uint32_t s0 = wave * per_wave, s1 = s0 + per_wave < steps ? s0 + per_wave : steps;
-    const uint8_t* code_at[R];
-    int64_t group_at[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        int64_t c = col0 + (gated ? r % (R > 1 ? R / 2 : 1) : r) * 16 + r16;
-        c = c < width ? c : width - 1;
-        if (gated && r >= R / 2) c += width;
-        const int64_t row = (int64_t)expert * n + c;
-        code_at[r] = a.codes + (four_bit(MODE) ? row * k / 2 : row * k);
-        group_at[r] = row * a.groups;
-    }
-    for (int64_t t0 = lo; t0 < hi; t0 += 16) {
-        const bool live = t0 + r16 < hi;
-        const uint16_t* xrow = (const uint16_t*)a.x + (live ? source_row(a.rows, t0 + r16) : 0) * a.ldx;
-        f32x4 acc[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r] = f32x4{0, 0, 0, 0};
-
-        FewStep<MODE, R> st[2];
-        auto load = [&](uint32_t s, FewStep<MODE, R>& d) {
-            uint32_t at = s * 128 + kq * 32;
-            const bool in = at < k;  // the last step may be short: its lanes read place 0 and count as zero through x
-            at = in ? at : 0;
-            const uint32_t v = at / 32, g = a.magic ? __umulhi(v, a.magic) : v;
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if constexpr (four_bit(MODE)) {
-                    d.codes[r][0] = *(const u32v4*)(code_at[r] + at / 2);
-                } else {
-                    d.codes[r][0] = *(const u32v4*)(code_at[r] + at);
-                    d.codes[r][1] = *(const u32v4*)(code_at[r] + at + 16);
-                }
-                const int64_t gi = group_at[r] + g;
-                if constexpr (MODE == NNCF_AMD_MXFP4) d.scale[r] = ((const uint8_t*)a.scale)[gi];
-                else d.scale[r] = ((const uint16_t*)a.scale)[gi];
-                d.scale[r] = in ? d.scale[r] : 0;
-                if constexpr (MODE == NNCF_AMD_INT4_ASYM) d.zero[r] = (uint32_t)(a.zp[gi >> 1] >> (4 * (gi & 1))) & 15u;
-                if constexpr (MODE == NNCF_AMD_INT8_ASYM) d.zero[r] = a.zp[gi];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d.x[j] = u32v4{0, 0, 0, 0};
-            if (live && in) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) d.x[j] = *(const u32v4*)(xrow + at + 8 * j);
-            }
+    const uint32_t k = a.k, steps = sh.steps;
+    const uint32_t row_bytes = four_bit(MODE) ? k / 2 : k;
+    // Blocks begin at different places of k and go round: all in step at one column, they would ask the few memory channels
+    // that hold it (rows are often a power of two apart).
+    const uint32_t turn = (blockIdx.x & 15) * steps >> 4;
+    auto stage_of = [&](uint32_t s) {
+        uint32_t t = s + turn;
+        t = t < steps ? t : t - steps;
+        return (t < steps ? t : 0) * sh.wk + wk;
+    };
+    // rows of W from a scalar origin; rows behind the last are held to it, strips behind the last read the last row
+    auto origin_of = [&](int w) {
+        const int64_t c = column_of(w);
+        return (int64_t)expert * n + (c < width ? c : width - 1) + (gated && (w & 1) ? width : 0);
+    };
+    auto held_row = [&](int w, int i) {
+        const int64_t left = width - 1 - column_of(w);
+        return (uint32_t)(left < 0 ? 0 : i < left ? i : left);
+    };
+    const uint8_t* codes0 = a.codes + origin_of(wn) * row_bytes;
+    bool fresh = true;  // the scales are not yet here
+    for (int64_t t0 = lo; t0 < hi; t0 += sh.rows) {
+        const int rows = (int)(hi - t0 < sh.rows ? hi - t0 : sh.rows);
+        // (the lane's number anew: what is computed from it must not be carried round this loop in registers)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int r16 = lane & 15, kq = lane >> 4;
+        const uint32_t lc = (lane & 7) * 16;
+        const uint32_t ra = held_row(wn, lane >> 3) * row_bytes, rb = held_row(wn, (lane >> 3) + 8) * row_bytes;
+        const int put = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 4)) << 4);  // rows lane / 8 and 8 further: (row >> 1) & 7
+        const int put8 = ((lane >> 3) + 8) * 128 + (((lane & 7) ^ ((lane >> 4) + 4)) << 4);
+        const int get = r16 * 128 + (kq & 1) * 8;
+        u32v4 codes[2][2];
+        auto load = [&](uint32_t s, int d) {  // step s of this wave: the parts of k take turns
+            uint32_t at = stage_of(s) * 128 + lc;
+            at = at < row_bytes ? at : 0;  // behind the end: the row's first codes, times x's zeros
+            codes[d][0] = __builtin_nontemporal_load((const u32v4*)(codes0 + (ra + at)));
+            codes[d][1] = __builtin_nontemporal_load((const u32v4*)(codes0 + (rb + at)));
         };
-        auto use = [&](const FewStep<MODE, R>& d) {
+        load(0, 0);
+        load(1, 1);
+        // this wave's loads of x: rows wn * XROWS + lane / (64 / XROWS), then WN * XROWS further; those behind the last are held to it
+        uint32_t x_src[XI];
+        int x_put[XI];
+        const int xc = lane & (64 / XROWS - 1);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const GroupPar<MODE> g = par_of<MODE>(d.scale[r], d.zero[r]);
+        for (int i = 0; i < XI; ++i) {
+            int r = (wn + i * sh.wn) * XROWS + lane / (64 / XROWS);
+            r = r < rows ? r : rows - 1;
+            x_src[i] = (uint32_t)(source_row(a.rows, t0 + r) * a.ldx);
+            x_put[i] = (wk * sh.rows + r) * sh.x_bytes + ((xc ^ (r & 7)) << 4);
+        }
+        u32v4 xr[XI];
+        auto load_x = [&](uint32_t s) {
+            uint32_t at = stage_of(s) * KS + xc * 8;
+            at = at < k ? at : 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    u32v4 w;
-                    if constexpr (four_bit(MODE)) w = dequant8<MODE, DT>(d.codes[r][0][j], 0, g, lut);
-                    else w = dequant8<MODE, DT>(d.codes[r][j >> 1][2 * (j & 1)], d.codes[r][j >> 1][2 * (j & 1) + 1], g, lut);
-                    acc[r] = mfma16<DT>(w, d.x[j], acc[r]);
-                }
-            }
+            for (int i = 0; i < XI; ++i) xr[i] = *(const u32v4*)((const uint16_t*)a.x + (x_src[i] + at));
         };
-        if (s0 < s1) {
-            load(s0, st[0]);
-            uint32_t s = s0;
-            for (; s + 2 < s1; s += 2) {
-                load(s + 1, st[1]);
-                use(st[0]);
-                load(s + 2, st[0]);
-                use(st[1]);
+        const int x_size = sh.buffers > 1 ? sh.wk * sh.rows * sh.x_bytes : 0;
+        auto put_x = [&](uint32_t s) {
+            if (stage_of(s) * KS + KS > k) {  // what lies behind the end of k counts as zero
+                const bool in = stage_of(s) * KS + xc * 8 < k;
+#pragma unroll
+                for (int i = 0; i < XI; ++i) xr[i] = in ? xr[i] : u32v4{0, 0, 0, 0};
             }
-            if (s + 1 < s1) {
-                load(s + 1, st[1]);
-                use(st[0]);
-                use(st[1]);
+#pragma unroll
+            for (int i = 0; i < XI; ++i) *(u32v4*)(xbuf + (s & 1) * x_size + x_put[i]) = xr[i];
+        };
+        load_x(0);
+        if (fresh) {
+            // many loads at a time: a loop over single ones would wait for each
+            auto put_scale = [&](int at, uint32_t v) { scales[at] = (scale_t)v; };
+            if (a.scales8) {  // rows of whole eight groups: 8 of them a thread
+                const uint32_t eights = a.groups / 8, all = sh.wn * 16 * eights;
+                for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 2 * blockDim.x) {
+                    u32v4 v[2];
+                    uint32_t at[2];
+                    int zat[2];
+                    u32v2 zv[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t i = i0 + u * blockDim.x < all ? i0 + u * blockDim.x : i0, r = __umulhi(i, a.scales8), e = i - r * eights;
+                        const int64_t g0 = (origin_of(r >> 4) + held_row(r >> 4, r & 15)) * a.groups + e * 8;
+                        if constexpr (sizeof(scale_t) == 1) {
+                            const u32v2 w = *(const u32v2*)((const uint8_t*)a.scale + g0);
+                            v[u] = u32v4{w.x, w.y, 0, 0};
+                        } else {
+                            v[u] = *(const u32v4*)((const uint16_t*)a.scale + g0);
+                        }
+                        if constexpr (MODE == NNCF_AMD_INT4_ASYM) zv[u].x = *(const uint32_t*)(a.zp + (g0 >> 1));
+                        if constexpr (MODE == NNCF_AMD_INT8_ASYM) zv[u] = *(const u32v2*)(a.zp + g0);
+                        at[u] = ((r >> 4) * sh.pitch + e * 8) * 16 + (r & 15);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const uint32_t w = sizeof(scale_t) == 1 ? v[u][j >> 2] >> (8 * (j & 3)) : v[u][j >> 1] >> (16 * (j & 1));
+                            put_scale(at[u] + j * 16, w);
+                            if constexpr (MODE == NNCF_AMD_INT4_ASYM) zeros[at[u] + j * 16] = (zv[u].x >> (4 * j)) & 15;
+                            if constexpr (MODE == NNCF_AMD_INT8_ASYM) zeros[at[u] + j * 16] = (uint8_t)(zv[u][j >> 2] >> (8 * (j & 3)));
+                        }
+                }
             } else {
-                use(st[0]);
+                for (uint32_t g0 = 0; g0 < a.groups; g0 += 4) {  // a thread per row: lanes follow the rows of W
+                    for (int r = threadIdx.x; r < sh.wn * 16; r += blockDim.x) {
+                        const int64_t row = (origin_of(r >> 4) + held_row(r >> 4, r & 15)) * a.groups;
+                        uint32_t v[4], z[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int64_t g = row + (g0 + j < a.groups ? g0 + j : a.groups - 1);
+                            v[j] = ((const scale_t*)a.scale)[g];
+                            if constexpr (MODE == NNCF_AMD_INT4_ASYM) z[j] = (a.zp[g >> 1] >> (4 * (g & 1))) & 15;
+                            if constexpr (MODE == NNCF_AMD_INT8_ASYM) z[j] = a.zp[g];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (g0 + j < a.groups) {
+                                put_scale(((r >> 4) * sh.pitch + g0 + j) * 16 + (r & 15), v[j]);
+                                if constexpr (ASYM) zeros[((r >> 4) * sh.pitch + g0 + j) * 16 + (r & 15)] = (uint8_t)z[j];
+                            }
+                    }
+                }
+            }
+            // an odd number of groups of 32 ends in half a quarter; the other half meets x's zeros
+            for (int r = threadIdx.x; r < sh.wn * 16; r += blockDim.x) {
+                put_scale(((r >> 4) * sh.pitch + a.groups) * 16 + (r & 15), 0);
+                if constexpr (ASYM) zeros[((r >> 4) * sh.pitch + a.groups) * 16 + (r & 15)] = 0;
             }
         }
+        fresh = false;
+        put_x(0);
+        load_x(1);
+        auto sync = [&] {  // LDS only: the loads stay on their way
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        sync();
+        const int xrow = r16 < rows ? r16 : rows - 1;  // rows behind the last: their columns are not stored
+        // x's 16-byte chunk of a quarter: its low three bits are permuted by the row; whole 128 bytes are added on top
+        uint32_t x_get[2];
 #pragma unroll
-        for (int r = 0; r < R; ++r) part[wave][r][lane] = acc[r];
-        __syncthreads();
-        if (wave < tiles) {
-            f32x4 s = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+        for (int h = 0; h < 2; ++h)
+            x_get[h] = (wk * sh.rows + xrow) * sh.x_bytes + (((MF == 2 ? kq * 2 + h : kq + 4 * h) ^ (xrow & 7)) << 4);
+        // a quarter lies in one group, the same for all lanes but with groups of 32 (4-bit codes), where it takes in two
+        const int group0 = (wn * sh.pitch + (MF == 2 && a.groups * 32 == k ? kq >> 1 : 0)) * 16 + r16;
+        f32x4 acc = {0, 0, 0, 0};
+        auto step = [&](uint32_t s, int d) {
+            *(u32v4*)(mine + put) = codes[d][0];
+            *(u32v4*)(mine + put8) = codes[d][1];
+            load(s + 2, d);
+            const char* xs = xbuf + (s & 1) * x_size;
 #pragma unroll
-            for (int w = 0; w < kFewWaves; ++w) {
-                s += part[w][wave][lane];
-                if (gated) u += part[w][(wave + R / 2) % R][lane];
+            for (int q = 0; q < 4; ++q) {
+                const uint32_t kk = stage_of(s) * KS + q * (KS / 4), at = __umulhi(kk / 16, a.magic);
+                const int gi = group0 + 16 * (int)(at < a.groups ? at : a.groups - 1);  // (behind the end of k: any)
+                const GroupPar<MODE> g = par_of<MODE>(scales[gi], ASYM ? zeros[gi] : 0);
+                const u32v2 c = *(const u32v2*)(mine + get + (((2 * q + (kq >> 1)) ^ (r16 >> 1)) << 4));
+                if constexpr (MF == 2) {
+                    const u32v4 x0 = *(const u32v4*)(xs + x_get[0] + q * 128), x1 = *(const u32v4*)(xs + x_get[1] + q * 128);
+                    acc = mfma16<DT>(dequant8<MODE, DT>(c.x, 0, g, lut), x0, acc);
+                    acc = mfma16<DT>(dequant8<MODE, DT>(c.y, 0, g, lut), x1, acc);
+                } else {
+                    const u32v4 x0 = *(const u32v4*)(xs + x_get[q & 1] + (q >> 1) * 128);
+                    acc = mfma16<DT>(dequant8<MODE, DT>(c.x, c.y, g, lut), x0, acc);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // interleaved further, the values need more registers than there are
             }
-            if (t0 + r16 < hi) {
-                const float sv[4] = {s.x, s.y, s.z, s.w}, uv[4] = {u.x, u.y, u.z, u.w};
-                finish4<DT>(a.ep, t0 + r16, col0 + wave * 16 + 4 * kq, sv, uv);
+            if (s + 1 < steps) {  // (uniform over the block)
+                put_x(s + 1);
+                load_x(s + 2);
+            }
+            sync();
+        };
+        uint32_t s = 0;
+        for (; s + 1 < steps; s += 2) {
+            step(s, 0);
+            step(s + 1, 1);
+        }
+        if (s < steps) step(s, 0);
+        f32x4* sums = (f32x4*)dyn;  // [wave][lane] 2 KiB apart; every wave is behind its last step
+        sums[wave * 128 + lane] = acc;
+        sync();
+        if (wk == 0 && !(gated && (wn & 1))) {
+            f32x4 v = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+#pragma unroll 4
+            for (int w = 0; w < sh.wk; ++w) {
+                v += sums[(wave + w) * 128 + lane];
+                if (gated) u += sums[(wave + sh.wk + w) * 128 + lane];
+            }
+            asm volatile("" : "+v"(lane));
+            const int r16 = lane & 15, kq = lane >> 4;
+            if (r16 < rows) {
+                const float vv[4] = {v.x, v.y, v.z, v.w}, uv[4] = {u.x, u.y, u.z, u.w};
+                finish4<DT>(a.ep, t0 + r16, column_of(wn) + 4 * kq, vv, uv);
             }
         }
-        __syncthreads();
+        sync();
     }
 }
 
-bool few_fits(int mode, int64_t k, int64_t gs, const void* codes) {
-    return k % 32 == 0 && gs % 32 == 0 && k <= (1 << 20) && ((uintptr_t)codes & 15) == 0 && mode <= NNCF_AMD_MXFP4;
+FewShape few_shape(int mode, int64_t k, int64_t groups, int wn, int wk, int rows) {
+    const bool four = four_bit(mode);
+    const int64_t stages = (k + (four ? 255 : 127)) / (four ? 256 : 128);
+    return FewShape{wn, wk, rows, stages > wk ? 2 : 1, (int)((stages + wk - 1) / wk), (65536 + wk - 1) / wk, (int)groups + 1,
+                    mode == NNCF_AMD_MXFP4 ? 1 : 2, mode == NNCF_AMD_INT4_ASYM || mode == NNCF_AMD_INT8_ASYM ? 1 : 0, four ? 512 : 256};
+}
+
+bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t sources, int64_t ldx) {
+    return k % 32 == 0 && (gs == k || gs % 64 == 0 || gs == 32) && k <= (1 << 20) && few_shape(mode, k, k / gs, 2, 1, 16).total() <= kFewLdsBytes && ((uintptr_t)codes & 15) == 0 && mode <= NNCF_AMD_MXFP4 &&
+           sources * ldx < ((int64_t)1 << 31);
+}
+
+template <int MODE, int DT, int XI>
+int few_start(const FewArgs& a, const FewShape& sh, int64_t blocks, hipStream_t s) {
+    static OncePerDevice once;
+    const int first = once.first_on_device();
+    if (first < 0 || (first && hipFuncSetAttribute((const void*)k_few_rows<MODE, DT, XI>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kFewLdsBytes) != hipSuccess)) {
+        if (first > 0) once.forget_current();
+        set_error("linear: LDS refused");
+        return NNCF_AMD_ERR_LAUNCH;
+    }
+    hipLaunchKernelGGL((k_few_rows<MODE, DT, XI>), dim3((unsigned)blocks, (unsigned)a.rows.experts), dim3(64 * sh.waves()), (size_t)sh.total(), s, a, sh);
+    return launch_status("linear");
+}
+
+template <int MODE, int DT>
+int few_go(const FewArgs& a, hipStream_t s) {
+    const bool gated = a.ep.act == kActSwiglu;
+    const int64_t strips = ((gated ? a.ep.n / 2 : a.ep.n) + 15) / 16 * (gated ? 2 : 1);
+    if (a.rows.experts > 65535) {
+        set_error("linear: too many experts");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    const int64_t stage = four_bit(MODE) ? 256 : 128, stages = (a.k + stage - 1) / stage;
+    const int rows = (int)(a.rows.rows < 16 ? a.rows.rows : 16);
+    // the shape with the fewest steps over all the rounds of blocks on 256 compute units; a round costs two more to start and end
+    const int per_load = four_bit(MODE) ? 2 : 4;
+    auto loads_of = [&](int wn) { return (rows + wn * per_load - 1) / (wn * per_load); };
+    FewShape best{};
+    int64_t best_cost = INT64_MAX;
+    for (int wn = gated ? 2 : 1; wn <= 8; wn += gated ? 2 : 1)
+        for (int wk = 1; wn * wk <= kFewWaves && wk <= stages; ++wk) {
+            const FewShape sh = few_shape(MODE, a.k, a.groups, wn, wk, rows);
+            if (sh.total() > kFewLdsBytes || (loads_of(wn) > 4 && wn * wk > kFewWaves / 2)) continue;
+            const int64_t per_cu = kFewWaves / sh.waves() < kFewLdsBytes / sh.total() ? kFewWaves / sh.waves() : kFewLdsBytes / sh.total();
+            const int64_t blocks = (strips + wn - 1) / wn * a.rows.experts;
+            const int64_t cost = (blocks + 256 * per_cu - 1) / (256 * per_cu) * ((stages + wk - 1) / wk + 2);
+            if (cost < best_cost) best_cost = cost, best = sh;
+        }
+    const int64_t blocks = (strips + best.wn - 1) / best.wn;
+    if (best_cost == INT64_MAX || blocks > 0x7fffffff) {
+        set_error("linear: weight too large");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    const int loads = loads_of(best.wn);
+    if (loads <= 1) return few_start<MODE, DT, 1>(a, best, blocks, s);
+    if (loads <= 2) return few_start<MODE, DT, 2>(a, best, blocks, s);
+    if (loads <= 4) return few_start<MODE, DT, 4>(a, best, blocks, s);
+    if constexpr (four_bit(MODE)) return few_start<MODE, DT, 8>(a, best, blocks, s);
+    return NNCF_AMD_ERR_UNSUPPORTED;
 }
 
 template <int DT>
 int few_typed(int mode, const FewArgs& a, hipStream_t s) {
-    const bool gated = a.ep.act == kActSwiglu;
-    const int64_t width = gated ? a.ep.n / 2 : a.ep.n;
-    const int64_t tiles = (width + 15) / 16;
-    // two tiles of rows per wave read x half as often; one where that would leave compute units without a block
-    const int r = gated || tiles * a.rows.experts >= 1024 ? 2 : 1;
-    const int64_t per = gated ? r / 2 : r;
-    const int64_t gx = (tiles + per - 1) / per;
-    if (gx > 0x7fffffff || a.rows.experts > 65535) {
-        set_error("linear: weight too large");
-        return NNCF_AMD_ERR_UNSUPPORTED;
-    }
-    const dim3 grid((unsigned)gx, (unsigned)a.rows.experts), block(64 * kFewWaves);
-#define GO(M)                                                                                  \
-    case M:                                                                                    \
-        if (r == 2) hipLaunchKernelGGL((k_few_rows<M, DT, 2>), grid, block, 0, s, a);          \
-        else hipLaunchKernelGGL((k_few_rows<M, DT, 1>), grid, block, 0, s, a);                 \
-        break;
     switch (mode) {
-        GO(NNCF_AMD_INT8_ASYM)
-        GO(NNCF_AMD_INT8_SYM)
-        GO(NNCF_AMD_INT4_ASYM)
-        GO(NNCF_AMD_INT4_SYM)
-        GO(NNCF_AMD_NF4)
-        GO(NNCF_AMD_MXFP4)
+        case NNCF_AMD_INT8_ASYM: return few_go<NNCF_AMD_INT8_ASYM, DT>(a, s);
+        case NNCF_AMD_INT8_SYM: return few_go<NNCF_AMD_INT8_SYM, DT>(a, s);
+        case NNCF_AMD_INT4_ASYM: return few_go<NNCF_AMD_INT4_ASYM, DT>(a, s);
+        case NNCF_AMD_INT4_SYM: return few_go<NNCF_AMD_INT4_SYM, DT>(a, s);
+        case NNCF_AMD_NF4: return few_go<NNCF_AMD_NF4, DT>(a, s);
+        default: return few_go<NNCF_AMD_MXFP4, DT>(a, s);
     }
-#undef GO
-    return launch_status("linear");
 }
 
 int few_launch(int dtype, int mode, const FewArgs& a, hipStream_t s) {
