@@ -421,7 +421,7 @@ int nncf_amd_gptq_dequant8(const int32_t* qweight, const int32_t* qzeros, const 
  *   workspace  : nncf_amd_compressed_linear_workspace bytes, aligned to 16 (0: none needed)
  */
 size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k,
-                                            const void* codes, int mode, int64_t group_size);
+                                            const void* codes, int mode, int64_t group_size, int activation);
 int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes,
                                int mode, int64_t group_size, const void* scale, const uint8_t* zero_point,
                                const void* bias, int activation, const void* residual, int64_t ldr, void* y, int64_t ldy,
@@ -433,7 +433,8 @@ int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m,
  * Values outside the buffers are held to their ends.
  */
 size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, int64_t sources, int gathered, int64_t rows, int64_t n,
-                                        int64_t k, const void* codes, int mode, int64_t group_size, int64_t experts);
+                                        int64_t k, const void* codes, int mode, int64_t group_size, int64_t experts,
+                                        int activation);
 int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int64_t sources, const int32_t* slots, int64_t topk,
                            const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k, const void* codes,
                            int mode, int64_t group_size, const void* scale, const uint8_t* zero_point, int activation,

@@ -83,12 +83,12 @@ SIGNATURES = {
     "nncf_amd_cholinv_block": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "nncf_amd_gptq_pack8": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_void_p]),
     "nncf_amd_compressed_linear_workspace": (c_size_t, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int,
-                                                        c_int64]),
+                                                        c_int64, c_int]),
     "nncf_amd_compressed_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int, c_int64,
                                            c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64,
                                            c_void_p, c_void_p, c_size_t, c_void_p]),
     "nncf_amd_expert_linear_workspace": (c_size_t, [c_void_p, c_int64, c_int64, c_int, c_int64, c_int64, c_int64, c_void_p,
-                                                    c_int, c_int64, c_int64]),
+                                                    c_int, c_int64, c_int64, c_int]),
     "nncf_amd_expert_linear": (c_int, [c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                                        c_int64, c_int64, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int, c_void_p,
                                        c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),

@@ -2,19 +2,21 @@
 // with k running along their rows; plain or grouped by expert.  Used where the rows of x are many enough that W is worth
 // decompressing once (wc_linear.hip), in both directions (the gradient takes W transposed).
 //
-// A block owns a tile of 64 * FA rows of W by 64 * FB rows of x, four waves in a 2 x 2 arrangement, each FA x FB
-// accumulators of v_mfma_f32_32x32x16 (W is the A operand: a lane ends with four consecutive columns of one row of y).
-// Both operands go global -> LDS by buffer DMA in stages of 32 k (64 bytes a row), four stages: one being read, three on
-// their way.  A row's 16-byte chunk c sits at chunk position c ^ ((row >> 1) & 3): eight consecutive lanes of a fragment read
-// eight rows and then touch all 32 banks once.  The DMA writes LDS linearly, so the permutation is applied to its source.
+// A block owns a tile of 32 * WI * FA rows of W by 32 * WJ * FB rows of x, WI x WJ waves, each FA x FB accumulators of
+// v_mfma_f32_32x32x16 (W is the A operand: a lane ends with four consecutive columns of one row of y).
+// Both operands go global -> LDS by buffer DMA in stages of 64 k: 128 bytes a row, whole lines (stages of 32 k ask for half
+// lines and fetch each of them twice: 1.0 PFLOP/s where this form reaches the figure at dense_typed).  Two stages: while one is
+// read the other one lands; a barrier in the last quarter of a stage frees it.  A row's 16-byte chunk c sits at chunk position
+// c ^ (row & 7): eight consecutive lanes of a fragment read eight rows and then touch all banks.  The DMA writes LDS linearly,
+// so the permutation is applied to its source.
 #include <type_traits>
 
 #include "wc_linear.h"
 
 namespace wc {
 
-constexpr int kStages = 4;
-constexpr int kRowBytes = 64;  // 32 k of 16 bits
+constexpr int kStages = 2;
+constexpr int kRowBytes = 128;  // 64 k of 16 bits
 
 // written out: through the builtin the compiler sees an LDS store of unknown address and waits for it at every LDS read
 __device__ __forceinline__ void dma16(const i32x4& rsrc, uint32_t voff, uint32_t soff, uint32_t lds) {
@@ -66,14 +68,15 @@ __device__ __forceinline__ bool find_tile(const RowMap& r, int64_t t, int& exper
     return false;
 }
 
-template <int DT, int FA, int FB>
-__global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, uint32_t tiles_n) {
-    constexpr int PA = 64 * FA, PB = 64 * FB;  // tile rows of W and of x
+template <int DT, int WI, int WJ, int FA, int FB>
+__global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, uint32_t tiles_n) {
+    constexpr int NW = WI * WJ, PA = 32 * WI * FA, PB = 32 * WJ * FB;  // waves; tile rows of W and of x
     constexpr int kStageBytes = (PA + PB) * kRowBytes;
-    constexpr int NDMA = FA + FB;  // DMA instructions per wave and stage: 16 rows each
+    constexpr int DA = PA / (8 * NW), DB = PB / (8 * NW), NDMA = DA + DB;  // DMA instructions per wave and stage: 8 rows each
+    static_assert(PA % (8 * NW) == 0 && PB % (8 * NW) == 0, "every wave brings in whole instructions' rows");
     extern __shared__ __align__(16) char smem[];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t wi = wave >> 1, wj = wave & 1;
+    const uint32_t wi = wave / WJ, wj = wave % WJ;
 
     // Tiles in bands of 8 row tiles, the row tile fastest inside a band; the workgroups of one XCD (they are dealt out in
     // turn over the 8 of them) take a run of consecutive tiles, so that its L2 holds 8 strips of x and a few of W.
@@ -94,7 +97,7 @@ __global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, 
         expert_range(g.rows, g.rows.experts - 1, lo, hi);
         const int64_t end = col0 + (gated ? PA / 2 : PA) < width ? col0 + (gated ? PA / 2 : PA) : width;
         for (int64_t r = hi + tm; r < g.rows.rows; r += tiles_m)
-            for (int64_t c = col0 + threadIdx.x; c < end; c += 256) {
+            for (int64_t c = col0 + threadIdx.x; c < end; c += 64 * NW) {
                 if (g.ep.y32) ((float*)g.ep.y)[r * g.ep.ldy + c] = 0.0f;
                 else ((uint16_t*)g.ep.y)[r * g.ep.ldy + c] = 0;
                 if (g.ep.z) {
@@ -107,7 +110,7 @@ __global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, 
     int64_t first, last;
     if (!find_tile<PB>(g.rows, tm, expert, first, last)) return;
 
-    // sources of this lane's DMA chunks: instruction u of the wave fills 16 consecutive tile rows
+    // sources of this lane's DMA chunks: instruction u of the wave fills 8 consecutive tile rows
     const char* wbase = (const char*)g.w + (int64_t)expert * g.ep.n * g.k * 2;
     const char* xbase = (const char*)g.x;
     int64_t worg = 0, xorg = 0;  // origins that keep the 32-bit offsets small
@@ -117,9 +120,9 @@ __global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, 
     uint32_t voff[NDMA], dst[NDMA];
 #pragma unroll
     for (int u = 0; u < NDMA; ++u) {
-        const bool is_w = u < FA;
-        const uint32_t row = (is_w ? u * 64 : (u - FA) * 64) + wave * 16 + (lane >> 2);  // row in the operand's tile
-        const uint32_t chunk = (lane & 3) ^ ((row >> 1) & 3);
+        const bool is_w = u < DA;
+        const uint32_t at8 = ((is_w ? u : u - DA) * NW + wave) * 8, row = at8 + (lane >> 3);  // row in the operand's tile
+        const uint32_t chunk = (lane & 7) ^ (row & 7);
         int64_t at;
         if (is_w) {
             int64_t c;
@@ -139,23 +142,23 @@ __global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, 
             at = (source_row(g.rows, r) - xorg) * g.ldx * 2;
         }
         voff[u] = (uint32_t)at + chunk * 16;
-        dst[u] = (is_w ? 0 : PA * kRowBytes) + ((is_w ? u * 64 : (u - FA) * 64) + wave * 16) * kRowBytes;
+        dst[u] = ((is_w ? 0 : PA) + at8) * kRowBytes;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-    const int nst = (int)(g.k / 32);
+    const int nst = (int)(g.k / 64);
     uint32_t so = 0, lds_st = 0;
     auto issue_prepare = [&](int st) {
         so = (uint32_t)st * kRowBytes;
         lds_st = lds0 + (uint32_t)(st % kStages) * kStageBytes;
     };
-    auto issue_one = [&](int u) { dma16(u < FA ? rw : rx, voff[u], so, lds_st + dst[u]); };
+    auto issue_one = [&](int u) { dma16(u < DA ? rw : rx, voff[u], so, lds_st + dst[u]); };
 
     typedef int op_t __attribute__((ext_vector_type(4)));
     const uint32_t r32 = lane & 31, kh = lane >> 5;
-    uint32_t offa[2], offb[2];  // per half of the stage; the fragments follow 32 rows apart (32 rows keep the permutation)
+    uint32_t offa[4], offb[4];  // per quarter of the stage; the fragments follow 32 rows apart (32 rows keep the permutation)
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-        const uint32_t at = r32 * kRowBytes + (((2 * ks + kh) ^ ((r32 >> 1) & 3)) * 16);
+    for (int ks = 0; ks < 4; ++ks) {
+        const uint32_t at = r32 * kRowBytes + (((2 * ks + kh) ^ (r32 & 7)) * 16);
         offa[ks] = wi * 32 * FA * kRowBytes + at;
         offb[ks] = (PA + wj * 32 * FB) * kRowBytes + at;
     }
@@ -173,129 +176,134 @@ __global__ __launch_bounds__(256) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, 
         else
             asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b) : "memory");
     };
-    auto wait_dma = [&](int stages) {  // until at most `stages` stages are on their way
-        if (stages >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NDMA) : "memory");
-        else if (stages == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NDMA) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    };
-    constexpr int NM = FA * FB;
-    constexpr int kBarrierAfter = FA + FB - 1 < NM - 1 ? FA + FB - 1 : NM - 1;
-    constexpr int kSlots = 2 * NM - (kBarrierAfter + 1);
-    constexpr int kSlotStep = kSlots / NDMA > 0 ? kSlots / NDMA : 1;
-    static_assert(kSlots >= NDMA, "a stage's DMA instructions go between the MFMAs behind the barrier");
+    constexpr int NM = FA * FB, NR = FA + FB;
+    constexpr int kSync = 1;                // MFMAs of a stage's last quarter in front of the barrier
+    constexpr int kFirst = NM - kSync - 1;  // DMA instructions of a stage that go into the last quarter before it; the rest follows
     op_t a0[FA], b0[FB], a1[FA], b1[FB];
-    // 16 k: the MFMAs on (ca, cb); between them the LDS reads of the next 16 k, in the first half of a stage the wait for the
-    // next stage and the barrier that also frees the buffer of the stage before, and behind it the DMA into that buffer
-    auto kstep = [&](const op_t* ca, const op_t* cb, op_t* na, op_t* nb, const char* img, auto ks, auto reads, auto sync, auto dma,
-                     int stages) {
-        constexpr bool READS = decltype(reads)::value, SYNC = decltype(sync)::value, DMA = decltype(dma)::value;
-        constexpr int KS = decltype(ks)::value;       // half of the stage that is read: 1 in the stage's first step, else 0
-        constexpr int SLOT0 = KS == 1 ? -(kBarrierAfter + 1) : NM - (kBarrierAfter + 1);
+    // 16 k: the MFMAs on (ca, cb) and between them the LDS reads of the next 16 k from `img`, quarter KS of its stage.  KS == 0
+    // means the last quarter of the stage before: first the barrier (the other stage has landed, and nobody reads this one any
+    // more), then the DMA of the stage after next into its place.  DMA: instructions of it that are issued here, from D0 on.
+    auto kstep = [&](const op_t* ca, const op_t* cb, op_t* na, op_t* nb, const char* img, auto ks, auto reads, auto d0, auto d1) {
+        constexpr bool READS = decltype(reads)::value;
+        constexpr int KS = decltype(ks)::value, D0 = decltype(d0)::value, D1 = decltype(d1)::value;
+        constexpr int R0 = KS == 0 && READS ? kSync + 1 : 0;  // MFMA behind which the reads begin
+        constexpr int kPerSlot = (NR + NM - R0 - 1) / (NM - R0);
+        constexpr int kDmaPerSlot = D1 > D0 ? (D1 - D0 + NM - R0 - 1) / (NM - R0) : 0;
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
             mfma(acc[i / FB][i % FB], ca[i / FB], cb[i % FB]);
-            if constexpr (READS) {
-                if (i < FA) na[i] = read_op(img, offa[KS] + i * 32 * kRowBytes);
-                else if (i < FA + FB) nb[i - FA] = read_op(img, offb[KS] + (i - FA) * 32 * kRowBytes);
-                if (i == NM - 1)  // few MFMAs: the rest of the reads
-#pragma unroll
-                    for (int j = NM; j < FA + FB; ++j) {
-                        if (j < FA) na[j] = read_op(img, offa[KS] + j * 32 * kRowBytes);
-                        else nb[j - FA] = read_op(img, offb[KS] + (j - FA) * 32 * kRowBytes);
-                    }
-            }
-            if constexpr (SYNC) {
-                if (i == kBarrierAfter) {
-                    wait_dma(stages);
+            if constexpr (KS == 0 && READS) {
+                if (i == kSync) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                     __builtin_amdgcn_s_barrier();
                 }
             }
-            if constexpr (DMA) {
-                const int slot = SLOT0 + i;
-                if (slot >= 0 && slot % kSlotStep == 0 && slot / kSlotStep < NDMA) issue_one(slot / kSlotStep);
+            if constexpr (READS) {
+#pragma unroll
+                for (int j = 0; j < kPerSlot; ++j) {
+                    const int r = (i - R0) * kPerSlot + j;
+                    if (i < R0 || r >= NR) continue;
+                    if (r < FA) na[r] = read_op(img, offa[KS] + r * 32 * kRowBytes);
+                    else nb[r - FA] = read_op(img, offb[KS] + (r - FA) * 32 * kRowBytes);
+                }
+            }
+            if constexpr (D1 > D0) {
+#pragma unroll
+                for (int j = 0; j < kDmaPerSlot; ++j) {
+                    const int u = D0 + (i - R0) * kDmaPerSlot + j;
+                    if (i >= R0 && u < D1) issue_one(u);
+                }
             }
         }
     };
     using T = std::true_type;
     using F = std::false_type;
-    using K0 = std::integral_constant<int, 0>;
-    using K1 = std::integral_constant<int, 1>;
-    for (int st = 0; st < kStages - 1 && st < nst; ++st) {
-        issue_prepare(st);
+#define N_(v) std::integral_constant<int, (v)>{}
+    constexpr int kHead = NDMA < 2 * kFirst ? (NDMA + 1) / 2 : kFirst;  // of a stage's DMA in the quarter behind the barrier
+    issue_prepare(0);
 #pragma unroll
-        for (int u = 0; u < NDMA; ++u) issue_one(u);
-    }
-    wait_dma((nst < kStages - 1 ? nst : kStages - 1) - 1);
+    for (int u = 0; u < NDMA; ++u) issue_one(u);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
+    if (nst > 1) {
+        issue_prepare(1);
+#pragma unroll
+        for (int u = 0; u < kHead; ++u) issue_one(u);
+    }
 #pragma unroll
     for (int m = 0; m < FA; ++m) a0[m] = read_op(smem, offa[0] + m * 32 * kRowBytes);
 #pragma unroll
     for (int m = 0; m < FB; ++m) b0[m] = read_op(smem, offb[0] + m * 32 * kRowBytes);
     int st = 0;
-    for (; st + kStages - 1 < nst; ++st) {
-        const char* img = smem + (st % kStages) * kStageBytes;
-        issue_prepare(st + kStages - 1);
-        kstep(a0, b0, a1, b1, img, K1{}, T{}, T{}, T{}, 1);
-        kstep(a1, b1, a0, b0, smem + ((st + 1) % kStages) * kStageBytes, K0{}, T{}, F{}, T{}, 0);
+    for (; st + 2 < nst; ++st) {
+        const char* img = smem + (st & 1) * kStageBytes;
+        kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(kHead), N_(NDMA));
+        kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
+        kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
+        issue_prepare(st + 2);
+        kstep(a1, b1, a0, b0, smem + ((st + 1) & 1) * kStageBytes, N_(0), T{}, N_(0), N_(kHead));
     }
-    for (; st + 1 < nst; ++st) {
-        const char* img = smem + (st % kStages) * kStageBytes;
-        kstep(a0, b0, a1, b1, img, K1{}, T{}, T{}, F{}, nst - 2 - st);
-        kstep(a1, b1, a0, b0, smem + ((st + 1) % kStages) * kStageBytes, K0{}, T{}, F{}, F{}, 0);
+    if (st + 1 < nst) {
+        const char* img = smem + (st & 1) * kStageBytes;
+        kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(kHead), N_(NDMA));
+        kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
+        kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
+        kstep(a1, b1, a0, b0, smem + ((st + 1) & 1) * kStageBytes, N_(0), T{}, N_(0), N_(0));
+        ++st;
     }
-    kstep(a0, b0, a1, b1, smem + (st % kStages) * kStageBytes, K1{}, T{}, F{}, F{}, 0);
-    kstep(a1, b1, a0, b0, smem, K0{}, F{}, F{}, F{}, 0);
+    const char* img = smem + (st & 1) * kStageBytes;
+    kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(0), N_(0));
+    kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
+    kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
+    kstep(a1, b1, a0, b0, img, N_(0), F{}, N_(0), N_(0));
+#undef N_
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMAs leave the pipe before the read-out
 
-    const int64_t row0 = first + wj * 32 * FB + r32;
+    // Through LDS, 32 rows of y at a time (a wave's own 32 x 32 FA floats, rows 16 bytes further apart than they are long), so
+    // that a row's columns are finished and stored side by side and the epilogue is in the program once per 32 rows.
+    constexpr int kPitch = 32 * FA + 4;
+    float* tile = (float*)smem + wave * 32 * kPitch;
+    __syncthreads();
+    const uint32_t cols = gated ? 16 * FA : 32 * FA;  // of y
+    const int64_t col_w = col0 + wi * cols;
 #pragma unroll
     for (int b = 0; b < FB; ++b) {
-        const int64_t row = row0 + b * 32;
-        if (row >= last) continue;
-        if (gated) {
 #pragma unroll
-            for (int a = 0; a < (FA + 1) / 2; ++a)
+        for (int a = 0; a < FA; ++a)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    float s[4], u[4];
-                    if constexpr (FA >= 2) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) s[i] = acc[a][b][4 * q + i], u[i] = acc[(a + FA / 2) % FA][b][4 * q + i];
-                    }
-                    finish4<DT>(g.ep, row, col0 + wi * 16 * FA + a * 32 + 8 * q + 4 * kh, s, u);
-                }
-        } else {
-#pragma unroll
-            for (int a = 0; a < FA; ++a)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    float s[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[i] = acc[a][b][4 * q + i];
-                    finish4<DT>(g.ep, row, col0 + wi * 32 * FA + a * 32 + 8 * q + 4 * kh, s, s);
-                }
+            for (int q = 0; q < 4; ++q)
+                *(f32x4*)(tile + r32 * kPitch + a * 32 + 8 * q + 4 * kh) =
+                    f32x4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
+        const int64_t row0 = first + wj * 32 * FB + b * 32;
+        for (uint32_t i = lane * 4; i < 32 * cols; i += 256) {  // (the wave's own floats: no barrier)
+            const uint32_t r = i / cols, c = i % cols;
+            if (row0 + r >= last) break;
+            const f32x4 s = *(const f32x4*)(tile + r * kPitch + c);
+            const f32x4 u = gated ? *(const f32x4*)(tile + r * kPitch + 16 * FA + c) : s;
+            const float sv[4] = {s.x, s.y, s.z, s.w}, uv[4] = {u.x, u.y, u.z, u.w};
+            finish4<DT>(g.ep, row0 + r, col_w + c, sv, uv);
         }
     }
 }
 
-template <int DT, int FA, int FB>
+template <int DT, int WI, int WJ, int FA, int FB>
 int dense_tiles(const DenseArgs& a, hipStream_t s) {
     static OncePerDevice once;
-    constexpr int kLds = kStages * 64 * (FA + FB) * kRowBytes;
+    constexpr int PA = 32 * WI * FA, PB = 32 * WJ * FB, kStageLds = kStages * (PA + PB) * kRowBytes;
+    constexpr int kTileLds = WI * WJ * 32 * (32 * FA + 4) * 4;  // the epilogue's floats take the stages' place
+    constexpr int kLds = kStageLds > kTileLds ? kStageLds : kTileLds;
     const int first = once.first_on_device();
     if (first < 0) {
         set_error("linear: no current device");
         return NNCF_AMD_ERR_LAUNCH;
     }
-    if (first && hipFuncSetAttribute((const void*)k_gemm_nt<DT, FA, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
+    if (first && hipFuncSetAttribute((const void*)k_gemm_nt<DT, WI, WJ, FA, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
         once.forget_current();
         set_error("linear: %d bytes of LDS refused", kLds);
         return NNCF_AMD_ERR_LAUNCH;
     }
     const bool gated = a.ep.act == kActSwiglu;
-    const int64_t width = gated ? a.ep.n / 2 : a.ep.n, per = gated ? 32 * FA : 64 * FA, pb = 64 * FB;
+    const int64_t width = gated ? a.ep.n / 2 : a.ep.n, per = gated ? PA / 2 : PA, pb = PB;
     const int64_t tiles_n = (width + per - 1) / per;
     // ragged groups: each may end inside a tile
     const int64_t groups = a.rows.offsets ? (a.rows.experts < a.rows.rows ? a.rows.experts : a.rows.rows) : 1;
@@ -305,7 +313,7 @@ int dense_tiles(const DenseArgs& a, hipStream_t s) {
         set_error("linear: too many tiles");
         return NNCF_AMD_ERR_UNSUPPORTED;
     }
-    hipLaunchKernelGGL((k_gemm_nt<DT, FA, FB>), dim3((unsigned)blocks), dim3(256), kLds, s, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
+    hipLaunchKernelGGL((k_gemm_nt<DT, WI, WJ, FA, FB>), dim3((unsigned)blocks), dim3(64 * WI * WJ), kLds, s, a, (uint32_t)tiles_m, (uint32_t)tiles_n);
     return launch_status("linear");
 }
 
@@ -314,9 +322,22 @@ bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gate
     return (gated ? n : 512) * k * 2 < kMost && (gathered ? sources : 512) * ldx * 2 < kMost;
 }
 
+// 256 x 256 tiles by eight waves (1.28 PFLOP/s on 4096 x 28672 x 8192, one block per compute unit) or 128 x 128 by four (0.98,
+// two blocks): whichever needs less time in rounds of blocks, a round of the small ones costing two thirds of one of the
+// large ones (2047 x 4096 x 4096: 128 large tiles 110 us, 512 small ones 90; 4096 x 4096 x 4096: 141 against 158).
+template <int DT>
+int dense_typed(const DenseArgs& a, hipStream_t s) {
+    const int64_t width = a.ep.n, groups = a.rows.offsets ? a.rows.experts : 1;
+    auto rounds = [&](int64_t tile, int64_t at_once) {
+        const int64_t rows = (a.rows.rows + tile - 1) / tile + (groups - 1) / 2;  // ragged groups: half a tile each on average
+        return ((width + tile - 1) / tile * rows + at_once - 1) / at_once;
+    };
+    if (3 * rounds(256, 256) <= 2 * rounds(128, 512)) return dense_tiles<DT, 2, 4, 4, 2>(a, s);
+    return dense_tiles<DT, 2, 2, 2, 2>(a, s);
+}
+
 int dense_launch(int dtype, const DenseArgs& a, hipStream_t s) {
-    if (dtype == NNCF_AMD_BF16) return dense_tiles<NNCF_AMD_BF16, 2, 2>(a, s);
-    return dense_tiles<NNCF_AMD_F16, 2, 2>(a, s);
+    return dtype == NNCF_AMD_BF16 ? dense_typed<NNCF_AMD_BF16>(a, s) : dense_typed<NNCF_AMD_F16>(a, s);
 }
 
 }  // namespace wc

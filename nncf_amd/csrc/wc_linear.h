@@ -287,7 +287,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
     }
 }
 
-// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 32 and 16-byte rows, w [experts * n, k]
+// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 64 and 16-byte rows, w [experts * n, k]
 struct DenseArgs {
     const void* x;
     const void* w;
@@ -310,8 +310,32 @@ struct FewArgs {
     uint32_t scales8;           // ceil(2^32 / (groups / 8)) where rows have whole eight groups, aligned in memory; else 0
     RowMap rows;
     Epilogue ep;
+    float* sums;                // [kz][rows][n], kz > 1
 };
+// A block's shape and its LDS: codes [wave][2 KiB] (at the end the waves' sums), x [buffer][part][row][512 bytes (8-bit codes:
+// 256)], scales [strip][group][16 rows], zero points.
+struct FewShape {
+    int wn, wk, rows, buffers;    // rows of x at a time
+    int lds_rows, tiles;          // and that LDS holds; tiles of 16 of them
+    int steps, per_wk;            // steps of a wave; ceil(2^16 / wk)
+    int kz;                       // blocks that share k: above 1 they leave fp32 sums [kz][rows][n] in the workspace
+    int pitch;                    // groups of a row, and one place more
+    int scale_bytes, zero_bytes;  // per group; zero_bytes 0: none
+    int x_bytes;                  // of a row and step
+    int64_t cost;                 // its time in units of 0.12 us
+    __host__ __device__ int waves() const { return wn * wk; }
+    __host__ __device__ int x() const { return waves() * 2048; }
+    __host__ __device__ int scales() const {  // the waves' sums take the place of codes and x
+        const int end = x() + buffers * wk * lds_rows * x_bytes, sums = waves() * tiles * 1024;
+        return end > sums ? end : sums;
+    }
+    __host__ __device__ int zeros() const { return scales() + (wn * 16 * pitch * scale_bytes + 15) / 16 * 16; }
+    __host__ __device__ int total() const { return zeros() + wn * 16 * pitch * zero_bytes; }
+};
+
 bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t sources, int64_t ldx);
-int few_launch(int dtype, int mode, const FewArgs& a, hipStream_t s);
+// the quickest shape for `rows` rows of x over `experts` weights (grouped: with row offsets)
+FewShape few_plan(int mode, int64_t n, int64_t k, int64_t groups, bool gated, int64_t rows, int64_t experts, bool grouped);
+int few_launch(int dtype, int mode, const FewArgs& a, const FewShape& sh, hipStream_t s);
 
 }  // namespace wc

@@ -8,10 +8,10 @@
 
 namespace wc {
 
-constexpr int64_t round32(int64_t v) { return (v + 31) / 32 * 32; }
+constexpr int64_t round64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // ---------------------------------------------------------------------------------- weight -> dense rows of the workspace
-// [experts * n, kp], kp = k rounded up to 32, the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  A block
+// [experts * n, kp], kp = k rounded up to 64, the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  A block
 // takes ROWS rows; a thread 8 consecutive weights of a row, whose place and group come from multiplications by 2^32 / d
 // (exact while the product of both factors is below 2^32: k up to 131072).  An expert without rows is left out.
 constexpr int kDequantRows = 8;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void k_dequant_rows_any(const uint8_t* __restr
 }
 
 // ------------------------------------------------------------------------- weight -> its transpose, for the gradient of x
-// [experts, k, np], np = n rounded up to 32, the tail zero: tiles of 64 x 64 turned round in LDS (rows padded by 4 bytes so
+// [experts, k, np], np = n rounded up to 64, the tail zero: tiles of 64 x 64 turned round in LDS (rows padded by 4 bytes so
 // that the columns that are written fall on different banks).
 template <int MODE, int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_dequant_transposed(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
@@ -195,7 +195,7 @@ bool aligned_groups(const Weight& w) {  // 8 consecutive weights of a row: one g
 
 template <int DT>
 int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
-    const int64_t kp = round32(w.k), total_rows = w.experts * w.n, groups = w.k / w.gs;
+    const int64_t kp = round64(w.k), total_rows = w.experts * w.n, groups = w.k / w.gs;
     const bool fast = aligned_groups(w);
     const int64_t blocks = fast ? (total_rows + kDequantRows - 1) / kDequantRows : (total_rows * kp + 255) / 256;
     if (blocks > 0x7fffffff) {
@@ -235,7 +235,7 @@ int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t
 
 template <int DT>
 int dequant_transposed(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
-    const int64_t np = round32(w.n), tn = (w.n + 63) / 64, tk = (w.k + 63) / 64;
+    const int64_t np = round64(w.n), tn = (w.n + 63) / 64, tk = (w.k + 63) / 64;
     if (tn > 0x7fffffff || tk > 65535 || w.experts > 65535) {
         set_error("linear: weight too large");
         return NNCF_AMD_ERR_UNSUPPORTED;
@@ -295,26 +295,41 @@ int check_pointers(const char* what, const Weight& w) {
 // What a call's workspace holds, one behind the other: the decompressed weight, the packed rows of x; and whether the product
 // runs on the codes themselves.
 struct Need {
-    size_t weight, pack;
+    size_t weight, pack;  // (the codes' product: the sums of blocks that share k in the weight's place)
     bool few;
+    FewShape shape;
     size_t total() const { return weight + pack; }
 };
-// rows per group up to which the codes are multiplied as they are
-constexpr int64_t kFewRows = 16;
-bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gathered) {
-    return k % 32 || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
+// The time of the other way, in the units of FewShape: the weight decompressed (2.6 bytes an element at 5 TB/s) and multiplied
+// by 128 x 128 or 256 x 256 tiles (1.1 and 1.7 us for 64 k of a round of blocks, the former 0.65 where half the blocks fill it).
+// 28672 x 8192: codes 144 us against 280 for 128 rows, 270 against 300 for 256, 520 against 365 for 512.
+int64_t dense_cost(const Weight& w, int64_t rows, bool grouped) {
+    auto blocks = [&](int64_t tile) { return ((w.n + tile - 1) / tile) * ((rows + tile - 1) / tile + (grouped ? (w.experts - 1) / 2 : 0)); };
+    const int64_t small = blocks(128), large = blocks(256), steps = (w.k + 63) / 64;
+    const double t128 = small <= 256 ? 0.65 : 1.1 * (double)((small + 511) / 512), t256 = 1.7 * (double)((large + 255) / 256);
+    const double us = (double)w.experts * (double)w.n * (double)w.k * 2.6 / 5.0e6 + (double)steps * (t128 < t256 ? t128 : t256) + 8.0;
+    return (int64_t)(us / 0.12);
 }
-Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows) {
-    Need d{(size_t)(w.experts * w.n * round32(w.k)) * 2, 0, false};
+bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gathered) {
+    return k % 64 || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
+}
+Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows, bool gated, bool grouped) {
+    Need d{(size_t)(w.experts * w.n * round64(w.k)) * 2, 0, false, {}};
     const bool copy = ldx % 8 || ((uintptr_t)x & 15);
-    d.few = rows <= kFewRows * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? round32(w.k) : ldx);
-    if (d.few) d.weight = 0;
-    if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round32(w.k)) * 2;
+    d.few = rows <= 1024 * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? round64(w.k) : ldx);
+    if (d.few) {
+        d.shape = few_plan(w.mode, w.n, w.k, w.k / w.gs, gated, rows, w.experts, grouped);
+        d.few = d.shape.cost < dense_cost(w, rows, grouped);
+    }
+    if (d.few) {
+        d.weight = d.shape.kz > 1 ? (size_t)(d.shape.kz * rows * w.n + 3) / 4 * 16 : 0;
+    }
+    if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round64(w.k)) * 2;
     return d;
 }
 Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
-    Need d{(size_t)(w.experts * w.k * round32(w.n)) * 2, 0, false};
-    if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * round32(w.n)) * 2;
+    Need d{(size_t)(w.experts * w.k * round64(w.n)) * 2, 0, false, {}};
+    if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * round64(w.n)) * 2;
     return d;
 }
 
@@ -326,7 +341,7 @@ int vec_of(const Epilogue& e) {
 }
 
 int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* pack, hipStream_t s) {
-    const int64_t kp = round32(k);
+    const int64_t kp = round64(k);
     if (rows.rows > 0x7fffffff) {
         set_error("linear: too many rows");
         return NNCF_AMD_ERR_UNSUPPORTED;
@@ -337,7 +352,7 @@ int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* p
 }
 
 int run_dense(int dtype, const void* x, int64_t ldx, int64_t k, const void* w, RowMap rows, Epilogue ep, uint16_t* pack, hipStream_t s) {
-    const int64_t kp = round32(k);
+    const int64_t kp = round64(k);
     if (must_pack(x, ldx, k, rows.sources, rows.slots != nullptr)) {
         const int st = pack_rows(x, ldx, k, rows, pack, s);
         if (st != NNCF_AMD_OK) return st;
@@ -368,7 +383,7 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
         set_error("%s: null or overlapping rows (ldx=%lld ldy=%lld)", what, (long long)ldx, (long long)ep.ldy);
         return NNCF_AMD_ERR_BAD_ARG;
     }
-    const Need need = forward_need(w, x, ldx, rows.sources, rows.slots != nullptr, rows.rows);
+    const Need need = forward_need(w, x, ldx, rows.sources, rows.slots != nullptr, rows.rows, ep.act == kActSwiglu, rows.offsets != nullptr);
     if (need.total() && (!ws || ws_bytes < need.total() || ((uintptr_t)ws & 15))) {
         set_error("%s: workspace of %zu bytes, aligned to 16, needed", what, need.total());
         return NNCF_AMD_ERR_WORKSPACE;
@@ -376,7 +391,7 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
     if (need.few) {
         RowMap map = rows;
         if (need.pack) {
-            st = pack_rows(x, ldx, w.k, map, (uint16_t*)ws, s);
+            st = pack_rows(x, ldx, w.k, map, (uint16_t*)((char*)ws + need.weight), s);
             if (st != NNCF_AMD_OK) return st;
         }
         const uint32_t g16 = (uint32_t)(w.gs / 16);  // at least 2: groups of whole 32
@@ -387,7 +402,7 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
         const uint32_t scales8 = eights ? (uint32_t)((((uint64_t)1 << 32) + groups / 8 - 1) / (groups / 8)) : 0;
         Epilogue e = ep;
         e.vec = vec_of(e);
-        return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, groups, magic, scales8, map, e}, s);
+        return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, groups, magic, scales8, map, e, (float*)ws}, need.shape, s);
     }
     uint16_t* dense = (uint16_t*)ws;
     st = dtype == NNCF_AMD_BF16 ? dequant_rows<NNCF_AMD_BF16>(w, rows, dense, s) : dequant_rows<NNCF_AMD_F16>(w, rows, dense, s);
@@ -432,11 +447,12 @@ int check_groups(const char* what, const int32_t* offsets, const int32_t* slots,
 }  // namespace wc
 
 extern "C" size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes,
-                                                       int mode, int64_t group_size) {
+                                                       int mode, int64_t group_size, int activation) {
     using namespace wc;
     if (m < 1 || n < 1 || k < 1) return 0;
     const Weight w{(const uint8_t*)codes, nullptr, nullptr, mode, n, k, group_size == -1 ? k : group_size, 1};
-    return forward_need(w, x, ldx, m, false, m).total();
+    if (w.gs < 1 || k % w.gs) return 0;  // (the call refuses it)
+    return forward_need(w, x, ldx, m, false, m, activation == kActSwiglu, false).total();
 }
 
 extern "C" int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes, int mode,
@@ -458,11 +474,12 @@ extern "C" int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx,
 }
 
 extern "C" size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, int64_t sources, int gathered, int64_t rows, int64_t n,
-                                                   int64_t k, const void* codes, int mode, int64_t group_size, int64_t experts) {
+                                                   int64_t k, const void* codes, int mode, int64_t group_size, int64_t experts, int activation) {
     using namespace wc;
     if (rows < 1 || n < 1 || k < 1 || experts < 1) return 0;
     const Weight w{(const uint8_t*)codes, nullptr, nullptr, mode, n, k, group_size == -1 ? k : group_size, experts};
-    return forward_need(w, x, ldx, sources, gathered != 0, rows).total();
+    if (w.gs < 1 || k % w.gs) return 0;  // (the call refuses it)
+    return forward_need(w, x, ldx, sources, gathered != 0, rows, activation == kActSwiglu, true).total();
 }
 
 extern "C" int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int64_t sources, const int32_t* slots, int64_t topk,

@@ -1,5 +1,5 @@
-// wc_linear_few.hip -- the product with a compressed weight for few rows of x (a token per sequence): up to 16 of them, or as many
-// per expert, at a time.  The codes (0.5-1 byte per weight) are read once and dequantised in registers.
+// wc_linear_few.hip -- the product with a compressed weight for few rows of x (a token per sequence, a small batch): up to 64 of
+// them, or as many per expert, at a time.  The codes (0.5-1 byte per weight) are read once and dequantised in registers.
 //
 // A block owns WN strips of 16 rows of W and cuts k into WK parts, one wave for each pair (up to 16), all in step; one block per
 // compute unit where the strips allow it, so that there is one start and one end.  A wave's step is 256 k (128 with 8-bit
@@ -32,23 +32,9 @@ __device__ __forceinline__ f32x4 mfma16(const u32v4& a, const u32v4& b, f32x4 c)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// A block's shape and its LDS: codes [wave][2 KiB] (at the end the waves' sums), x [buffer][part][row][512 bytes (8-bit codes:
-// 256)], scales [strip][group][16 rows], zero points.
-struct FewShape {
-    int wn, wk, rows, buffers;    // rows of x at a time
-    int steps, per_wk;            // steps of a wave; ceil(2^16 / wk)
-    int pitch;                    // groups of a row, and one place more
-    int scale_bytes, zero_bytes;  // per group; zero_bytes 0: none
-    int x_bytes;                  // of a row and step
-    __host__ __device__ int waves() const { return wn * wk; }
-    __host__ __device__ int x() const { return waves() * 2048; }
-    __host__ __device__ int scales() const { return x() + buffers * wk * rows * x_bytes; }
-    __host__ __device__ int zeros() const { return scales() + (wn * 16 * pitch * scale_bytes + 15) / 16 * 16; }
-    __host__ __device__ int total() const { return zeros() + wn * 16 * pitch * zero_bytes; }
-};
-
-// XI: loads of two rows of x (8-bit codes: four) that a wave makes per step; 8 of them need the registers of 16 waves for 8
-template <int MODE, int DT, int XI>
+// TT: tiles of 16 rows of x.  XI: loads of two rows of x (8-bit codes: four) that a wave makes per step; 8 of them need the
+// registers of 16 waves for 8.
+template <int MODE, int DT, int TT, int XI>
 __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_rows(FewArgs a, FewShape sh) {
     constexpr int MF = four_bit(MODE) ? 2 : 1;           // matrix instructions per 8 bytes of codes
     constexpr uint32_t KS = four_bit(MODE) ? 256 : 128;  // k of a step
@@ -70,7 +56,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
     // strip w of the block: 16 columns of y; with a gate the even ones are the gate's rows, the odd ones the other half's
     auto column_of = [&](int w) { return gated ? ((int64_t)blockIdx.x * (sh.wn / 2) + (w >> 1)) * 16 : ((int64_t)blockIdx.x * sh.wn + w) * 16; };
     int64_t lo, hi;
-    if (a.rows.offsets && expert == 0) {  // rows behind the last group are zero
+    if (a.rows.offsets && expert == 0 && blockIdx.z == 0) {  // rows behind the last group are zero
         expert_range(a.rows, a.rows.experts - 1, lo, hi);
         const int64_t c0 = column_of(0), c1 = c0 + (gated ? sh.wn / 2 : sh.wn) * 16 < width ? c0 + (gated ? sh.wn / 2 : sh.wn) * 16 : width;
         for (int64_t r = hi + wave; r < a.rows.rows; r += sh.waves())
@@ -93,7 +79,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
     auto stage_of = [&](uint32_t s) {
         uint32_t t = s + turn;
         t = t < steps ? t : t - steps;
-        return (t < steps ? t : 0) * sh.wk + wk;
+        return (blockIdx.z * steps + (t < steps ? t : 0)) * sh.wk + wk;
     };
     // rows of W from a scalar origin; rows behind the last are held to it, strips behind the last read the last row
     auto origin_of = [&](int w) {
@@ -135,7 +121,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
             int r = (wn + i * sh.wn) * XROWS + lane / (64 / XROWS);
             r = r < rows ? r : rows - 1;
             x_src[i] = (uint32_t)(source_row(a.rows, t0 + r) * a.ldx);
-            x_put[i] = (wk * sh.rows + r) * sh.x_bytes + ((xc ^ (r & 7)) << 4);
+            x_put[i] = (wk * sh.lds_rows + r) * sh.x_bytes + ((xc ^ (r & 7)) << 4);
         }
         u32v4 xr[XI];
         auto load_x = [&](uint32_t s) {
@@ -144,7 +130,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
 #pragma unroll
             for (int i = 0; i < XI; ++i) xr[i] = *(const u32v4*)((const uint16_t*)a.x + (x_src[i] + at));
         };
-        const int x_size = sh.buffers > 1 ? sh.wk * sh.rows * sh.x_bytes : 0;
+        const int x_size = sh.buffers > 1 ? sh.wk * sh.lds_rows * sh.x_bytes : 0;
         auto put_x = [&](uint32_t s) {
             if (stage_of(s) * KS + KS > k) {  // what lies behind the end of k counts as zero
                 const bool in = stage_of(s) * KS + xc * 8 < k;
@@ -225,15 +211,19 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
             asm volatile("" ::: "memory");
         };
         sync();
-        const int xrow = r16 < rows ? r16 : rows - 1;  // rows behind the last: their columns are not stored
+        // rows behind the last: their columns are not stored (what LDS holds there reaches nothing else)
+        const int xrow = TT > 1 || r16 < rows ? r16 : rows - 1;
         // x's 16-byte chunk of a quarter: its low three bits are permuted by the row; whole 128 bytes are added on top
         uint32_t x_get[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-            x_get[h] = (wk * sh.rows + xrow) * sh.x_bytes + (((MF == 2 ? kq * 2 + h : kq + 4 * h) ^ (xrow & 7)) << 4);
+            x_get[h] = (wk * sh.lds_rows + xrow) * sh.x_bytes + (((MF == 2 ? kq * 2 + h : kq + 4 * h) ^ (xrow & 7)) << 4);
         // a quarter lies in one group, the same for all lanes but with groups of 32 (4-bit codes), where it takes in two
         const int group0 = (wn * sh.pitch + (MF == 2 && a.groups * 32 == k ? kq >> 1 : 0)) * 16 + r16;
-        f32x4 acc = {0, 0, 0, 0};
+        f32x4 acc[TT];
+#pragma unroll
+        for (int j = 0; j < TT; ++j) acc[j] = f32x4{0, 0, 0, 0};
+        constexpr int kTile = 16 * (four_bit(MODE) ? 512 : 256);  // bytes of 16 rows of x
         auto step = [&](uint32_t s, int d) {
             *(u32v4*)(mine + put) = codes[d][0];
             *(u32v4*)(mine + put8) = codes[d][1];
@@ -246,12 +236,16 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
                 const GroupPar<MODE> g = par_of<MODE>(scales[gi], ASYM ? zeros[gi] : 0);
                 const u32v2 c = *(const u32v2*)(mine + get + (((2 * q + (kq >> 1)) ^ (r16 >> 1)) << 4));
                 if constexpr (MF == 2) {
-                    const u32v4 x0 = *(const u32v4*)(xs + x_get[0] + q * 128), x1 = *(const u32v4*)(xs + x_get[1] + q * 128);
-                    acc = mfma16<DT>(dequant8<MODE, DT>(c.x, 0, g, lut), x0, acc);
-                    acc = mfma16<DT>(dequant8<MODE, DT>(c.y, 0, g, lut), x1, acc);
+                    const u32v4 w0 = dequant8<MODE, DT>(c.x, 0, g, lut), w1 = dequant8<MODE, DT>(c.y, 0, g, lut);
+#pragma unroll
+                    for (int j = 0; j < TT; ++j) {
+                        acc[j] = mfma16<DT>(w0, *(const u32v4*)(xs + x_get[0] + q * 128 + j * kTile), acc[j]);
+                        acc[j] = mfma16<DT>(w1, *(const u32v4*)(xs + x_get[1] + q * 128 + j * kTile), acc[j]);
+                    }
                 } else {
-                    const u32v4 x0 = *(const u32v4*)(xs + x_get[q & 1] + (q >> 1) * 128);
-                    acc = mfma16<DT>(dequant8<MODE, DT>(c.x, c.y, g, lut), x0, acc);
+                    const u32v4 w0 = dequant8<MODE, DT>(c.x, c.y, g, lut);
+#pragma unroll
+                    for (int j = 0; j < TT; ++j) acc[j] = mfma16<DT>(w0, *(const u32v4*)(xs + x_get[q & 1] + (q >> 1) * 128 + j * kTile), acc[j]);
                 }
                 __builtin_amdgcn_sched_barrier(0);  // interleaved further, the values need more registers than there are
             }
@@ -267,104 +261,197 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
             step(s + 1, 1);
         }
         if (s < steps) step(s, 0);
-        f32x4* sums = (f32x4*)dyn;  // [wave][lane] 2 KiB apart; every wave is behind its last step
-        sums[wave * 128 + lane] = acc;
+        f32x4* sums = (f32x4*)dyn;  // [wave][tile][lane]; every wave is behind its last step
+#pragma unroll
+        for (int j = 0; j < TT; ++j) sums[(wave * TT + j) * 64 + lane] = acc[j];
         sync();
-        if (wk == 0 && !(gated && (wn & 1))) {
-            f32x4 v = {0, 0, 0, 0}, u = {0, 0, 0, 0};
-#pragma unroll 4
-            for (int w = 0; w < sh.wk; ++w) {
-                v += sums[(wave + w) * 128 + lane];
-                if (gated) u += sums[(wave + sh.wk + w) * 128 + lane];
-            }
+        if (!(gated && (wn & 1))) {
             asm volatile("" : "+v"(lane));
             const int r16 = lane & 15, kq = lane >> 4;
-            if (r16 < rows) {
-                const float vv[4] = {v.x, v.y, v.z, v.w}, uv[4] = {u.x, u.y, u.z, u.w};
-                finish4<DT>(a.ep, t0 + r16, column_of(wn) + 4 * kq, vv, uv);
+            for (int j = wk; j < TT; j += sh.wk) {
+                if (16 * j >= rows) break;
+                f32x4 v = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+#pragma unroll 4
+                for (int w = 0; w < sh.wk; ++w) {
+                    v += sums[((wn * sh.wk + w) * TT + j) * 64 + lane];
+                    if (gated) u += sums[(((wn + 1) * sh.wk + w) * TT + j) * 64 + lane];
+                }
+                if (16 * j + r16 < rows) {
+                    const float vv[4] = {v.x, v.y, v.z, v.w}, uv[4] = {u.x, u.y, u.z, u.w};
+                    const int64_t row = t0 + 16 * j + r16, col = column_of(wn) + 4 * kq;
+                    if (sh.kz == 1) {
+                        finish4<DT>(a.ep, row, col, vv, uv);
+                    } else {
+                        float* to = a.sums + ((int64_t)blockIdx.z * a.rows.rows + row) * n + col;
+                        for (int i = 0; i < 4 && col + i < width; ++i) {
+                            to[i] = vv[i];
+                            if (gated) to[width + i] = uv[i];
+                        }
+                    }
+                }
             }
         }
         sync();
     }
 }
 
-FewShape few_shape(int mode, int64_t k, int64_t groups, int wn, int wk, int rows) {
+// the blocks' sums over the parts of k, in their order, and the epilogue: a thread per 4 columns of a row
+template <int DT>
+__global__ __launch_bounds__(256) void k_few_join(const float* __restrict__ sums, int kz, RowMap rows, Epilogue ep) {
+    const int64_t width = ep.act == kActSwiglu ? ep.n / 2 : ep.n;
+    const int64_t quads = (width + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t lo, end = rows.rows;
+    if (rows.offsets) expert_range(rows, rows.experts - 1, lo, end);
+    const int64_t row = i / quads, col = (i - row * quads) * 4;
+    if (row >= end) return;  // (rows behind the last group have their zeros)
+    float s[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
+    for (int z = 0; z < kz; ++z) {
+        const float* from = sums + ((int64_t)z * rows.rows + row) * ep.n + col;
+        if (col + 4 <= width && ep.n % 4 == 0 && width % 4 == 0) {
+            const f32x4 v = *(const f32x4*)from;
+            s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+            if (ep.act == kActSwiglu) {
+                const f32x4 w = *(const f32x4*)(from + width);
+                u[0] += w.x, u[1] += w.y, u[2] += w.z, u[3] += w.w;
+            }
+        } else {
+            for (int j = 0; j < 4 && col + j < width; ++j) {
+                s[j] += from[j];
+                if (ep.act == kActSwiglu) u[j] += from[width + j];
+            }
+        }
+    }
+    finish4<DT>(ep, row, col, s, u);
+}
+
+FewShape few_shape(int mode, int64_t k, int64_t groups, int wn, int wk, int kz, int rows, int tiles) {
     const bool four = four_bit(mode);
     const int64_t stages = (k + (four ? 255 : 127)) / (four ? 256 : 128);
-    return FewShape{wn, wk, rows, stages > wk ? 2 : 1, (int)((stages + wk - 1) / wk), (65536 + wk - 1) / wk, (int)groups + 1,
-                    mode == NNCF_AMD_MXFP4 ? 1 : 2, mode == NNCF_AMD_INT4_ASYM || mode == NNCF_AMD_INT8_ASYM ? 1 : 0, four ? 512 : 256};
+    const int steps = (int)((stages + (int64_t)wk * kz - 1) / ((int64_t)wk * kz));
+    return FewShape{wn, wk, rows, steps > 1 ? 2 : 1, tiles > 1 ? 16 * tiles : rows, tiles, steps, (65536 + wk - 1) / wk, kz, (int)groups + 1,
+                    mode == NNCF_AMD_MXFP4 ? 1 : 2, mode == NNCF_AMD_INT4_ASYM || mode == NNCF_AMD_INT8_ASYM ? 1 : 0, four ? 512 : 256, 0};
+}
+
+int few_loads(int mode, const FewShape& sh) {  // of x, per wave and step
+    const int per_load = four_bit(mode) ? 2 : 4;
+    return (sh.rows + sh.wn * per_load - 1) / (sh.wn * per_load);
 }
 
 bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t sources, int64_t ldx) {
-    return k % 32 == 0 && (gs == k || gs % 64 == 0 || gs == 32) && k <= (1 << 20) && few_shape(mode, k, k / gs, 2, 1, 16).total() <= kFewLdsBytes && ((uintptr_t)codes & 15) == 0 && mode <= NNCF_AMD_MXFP4 &&
+    return k % 32 == 0 && (gs == k || gs % 64 == 0 || gs == 32) && k <= (1 << 20) && few_shape(mode, k, k / gs, 2, 1, 1, 16, 1).total() <= kFewLdsBytes && ((uintptr_t)codes & 15) == 0 && mode <= NNCF_AMD_MXFP4 &&
            sources * ldx < ((int64_t)1 << 31);
 }
 
-template <int MODE, int DT, int XI>
-int few_start(const FewArgs& a, const FewShape& sh, int64_t blocks, hipStream_t s) {
+static FewShape search(int mode, int64_t n, int64_t k, int64_t groups, bool gated, int64_t rows, int64_t experts, bool grouped) {
+    const int64_t strips = ((gated ? n / 2 : n) + 15) / 16 * (gated ? 2 : 1);
+    const int64_t stage = four_bit(mode) ? 256 : 128, stages = (k + stage - 1) / stage;
+    // rows per group: with experts the mean, a quarter more for their spread
+    const int64_t most = grouped ? (rows < 16 ? rows : (5 * rows / experts + 3) / 4) : rows;
+    FewShape best{};
+    best.cost = INT64_MAX;
+    for (int tiles = 1; tiles <= 4; tiles *= 2) {
+        if (tiles > 1 && most <= 8 * tiles) break;
+        const int64_t passes = (most + 16 * tiles - 1) / (16 * tiles);
+        const int64_t held = grouped ? (rows < 16 * tiles ? rows : 16 * tiles) : (rows + passes - 1) / passes;  // passes of equal length
+        for (int wn = gated ? 2 : 1; wn <= 8; wn += gated ? 2 : 1)
+            for (int wk = 1; wn * wk <= kFewWaves && wk <= stages; ++wk)
+                for (int kz = 1; kz <= 16 && (kz == 1 || kz * wk <= stages); kz += kz < 4 ? 1 : kz < 8 ? 2 : 4) {
+                    const FewShape sh = few_shape(mode, k, groups, wn, wk, kz, (int)held, tiles);
+                    const int loads = few_loads(mode, sh);
+                    if (sh.total() > kFewLdsBytes || loads > 8 || (loads > 4 && wn * wk > kFewWaves / 2)) continue;
+                    // In units of 0.12 us, from 28672 x 8192 and 4096 x 4096: a step takes 6 and 1 for every wave on the compute unit,
+                    // a tenth more with two tiles of x and six tenths with four; a round of blocks 40 to start and end; the join
+                    // of kz blocks 25 and its bytes.
+                    const int waves_fit = kFewWaves / sh.waves(), lds_fit = kFewLdsBytes / sh.total();
+                    const int64_t blocks = (strips + wn - 1) / wn * experts * kz;
+                    int64_t per_cu = waves_fit < lds_fit ? waves_fit : lds_fit;
+                    const int64_t rounds = (blocks + 256 * per_cu - 1) / (256 * per_cu);
+                    if (blocks < 256 * per_cu) per_cu = (blocks + 255) / 256;
+                    const int64_t step = (6 + per_cu * sh.waves()) * (tiles == 1 ? 10 : tiles == 2 ? 11 : 16);
+                    int64_t cost = rounds * (passes * (sh.steps + 1) * step / 10 + 40);
+                    if (kz > 1) cost += 25 + kz * rows * n / 60000;
+                    if (cost < best.cost) best = sh, best.cost = cost;
+                }
+    }
+    return best;
+}
+
+// The search takes tens of microseconds; its answers depend on these numbers alone and are kept, per thread.
+FewShape few_plan(int mode, int64_t n, int64_t k, int64_t groups, bool gated, int64_t rows, int64_t experts, bool grouped) {
+    struct Known {
+        int64_t key[7];
+        FewShape shape;
+    };
+    static thread_local Known known[64];
+    const int64_t key[7] = {n, k, groups, rows, experts, mode * 4 + gated * 2 + grouped, 1};
+    uint64_t h = 0;
+    for (int64_t v : key) h = (h ^ (uint64_t)v) * 0x9e3779b97f4a7c15ull, h ^= h >> 29;
+    Known& at = known[h & 63];
+    for (int i = 0; i < 7; ++i)
+        if (at.key[i] != key[i]) {
+            at.shape = search(mode, n, k, groups, gated, rows, experts, grouped);
+            for (int j = 0; j < 7; ++j) at.key[j] = key[j];
+            break;
+        }
+    return at.shape;
+}
+
+template <int MODE, int DT, int TT, int XI>
+int few_start(const FewArgs& a, const FewShape& sh, hipStream_t s) {
     static OncePerDevice once;
+    const bool gated = a.ep.act == kActSwiglu;
+    const int64_t width = gated ? a.ep.n / 2 : a.ep.n, strips = (width + 15) / 16 * (gated ? 2 : 1);
+    const int64_t blocks = (strips + sh.wn - 1) / sh.wn;
     const int first = once.first_on_device();
-    if (first < 0 || (first && hipFuncSetAttribute((const void*)k_few_rows<MODE, DT, XI>, hipFuncAttributeMaxDynamicSharedMemorySize,
+    if (first < 0 || (first && hipFuncSetAttribute((const void*)k_few_rows<MODE, DT, TT, XI>, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                    kFewLdsBytes) != hipSuccess)) {
         if (first > 0) once.forget_current();
         set_error("linear: LDS refused");
         return NNCF_AMD_ERR_LAUNCH;
     }
-    hipLaunchKernelGGL((k_few_rows<MODE, DT, XI>), dim3((unsigned)blocks, (unsigned)a.rows.experts), dim3(64 * sh.waves()), (size_t)sh.total(), s, a, sh);
+    if (blocks > 0x7fffffff || a.rows.experts > 65535) {
+        set_error("linear: weight too large");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    const dim3 grid((unsigned)blocks, (unsigned)a.rows.experts, (unsigned)sh.kz);
+    hipLaunchKernelGGL((k_few_rows<MODE, DT, TT, XI>), grid, dim3(64 * sh.waves()), (size_t)sh.total(), s, a, sh);
+    const int st = launch_status("linear");
+    if (st != NNCF_AMD_OK || sh.kz == 1) return st;
+    const int64_t join = ((width + 3) / 4 * a.rows.rows + 255) / 256;
+    if (join > 0x7fffffff) {
+        set_error("linear: too many rows");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    hipLaunchKernelGGL((k_few_join<DT>), dim3((unsigned)join), dim3(256), 0, s, a.sums, sh.kz, a.rows, a.ep);
     return launch_status("linear");
 }
 
 template <int MODE, int DT>
-int few_go(const FewArgs& a, hipStream_t s) {
-    const bool gated = a.ep.act == kActSwiglu;
-    const int64_t strips = ((gated ? a.ep.n / 2 : a.ep.n) + 15) / 16 * (gated ? 2 : 1);
-    if (a.rows.experts > 65535) {
-        set_error("linear: too many experts");
-        return NNCF_AMD_ERR_UNSUPPORTED;
+int few_go(const FewArgs& a, const FewShape& sh, hipStream_t s) {
+    const int loads = few_loads(MODE, sh);
+    if (sh.tiles == 1) {
+        if (loads <= 1) return few_start<MODE, DT, 1, 1>(a, sh, s);
+        if (loads <= 4) return few_start<MODE, DT, 1, 4>(a, sh, s);
+        return few_start<MODE, DT, 1, 8>(a, sh, s);
     }
-    const int64_t stage = four_bit(MODE) ? 256 : 128, stages = (a.k + stage - 1) / stage;
-    const int rows = (int)(a.rows.rows < 16 ? a.rows.rows : 16);
-    // the shape with the fewest steps over all the rounds of blocks on 256 compute units; a round costs two more to start and end
-    const int per_load = four_bit(MODE) ? 2 : 4;
-    auto loads_of = [&](int wn) { return (rows + wn * per_load - 1) / (wn * per_load); };
-    FewShape best{};
-    int64_t best_cost = INT64_MAX;
-    for (int wn = gated ? 2 : 1; wn <= 8; wn += gated ? 2 : 1)
-        for (int wk = 1; wn * wk <= kFewWaves && wk <= stages; ++wk) {
-            const FewShape sh = few_shape(MODE, a.k, a.groups, wn, wk, rows);
-            if (sh.total() > kFewLdsBytes || (loads_of(wn) > 4 && wn * wk > kFewWaves / 2)) continue;
-            const int64_t per_cu = kFewWaves / sh.waves() < kFewLdsBytes / sh.total() ? kFewWaves / sh.waves() : kFewLdsBytes / sh.total();
-            const int64_t blocks = (strips + wn - 1) / wn * a.rows.experts;
-            const int64_t cost = (blocks + 256 * per_cu - 1) / (256 * per_cu) * ((stages + wk - 1) / wk + 2);
-            if (cost < best_cost) best_cost = cost, best = sh;
-        }
-    const int64_t blocks = (strips + best.wn - 1) / best.wn;
-    if (best_cost == INT64_MAX || blocks > 0x7fffffff) {
-        set_error("linear: weight too large");
-        return NNCF_AMD_ERR_UNSUPPORTED;
-    }
-    const int loads = loads_of(best.wn);
-    if (loads <= 1) return few_start<MODE, DT, 1>(a, best, blocks, s);
-    if (loads <= 2) return few_start<MODE, DT, 2>(a, best, blocks, s);
-    if (loads <= 4) return few_start<MODE, DT, 4>(a, best, blocks, s);
-    if constexpr (four_bit(MODE)) return few_start<MODE, DT, 8>(a, best, blocks, s);
-    return NNCF_AMD_ERR_UNSUPPORTED;
+    if (sh.tiles == 2) return loads <= 4 ? few_start<MODE, DT, 2, 4>(a, sh, s) : few_start<MODE, DT, 2, 8>(a, sh, s);
+    return loads <= 4 ? few_start<MODE, DT, 4, 4>(a, sh, s) : few_start<MODE, DT, 4, 8>(a, sh, s);
 }
 
 template <int DT>
-int few_typed(int mode, const FewArgs& a, hipStream_t s) {
+int few_typed(int mode, const FewArgs& a, const FewShape& sh, hipStream_t s) {
     switch (mode) {
-        case NNCF_AMD_INT8_ASYM: return few_go<NNCF_AMD_INT8_ASYM, DT>(a, s);
-        case NNCF_AMD_INT8_SYM: return few_go<NNCF_AMD_INT8_SYM, DT>(a, s);
-        case NNCF_AMD_INT4_ASYM: return few_go<NNCF_AMD_INT4_ASYM, DT>(a, s);
-        case NNCF_AMD_INT4_SYM: return few_go<NNCF_AMD_INT4_SYM, DT>(a, s);
-        case NNCF_AMD_NF4: return few_go<NNCF_AMD_NF4, DT>(a, s);
-        default: return few_go<NNCF_AMD_MXFP4, DT>(a, s);
+        case NNCF_AMD_INT8_ASYM: return few_go<NNCF_AMD_INT8_ASYM, DT>(a, sh, s);
+        case NNCF_AMD_INT8_SYM: return few_go<NNCF_AMD_INT8_SYM, DT>(a, sh, s);
+        case NNCF_AMD_INT4_ASYM: return few_go<NNCF_AMD_INT4_ASYM, DT>(a, sh, s);
+        case NNCF_AMD_INT4_SYM: return few_go<NNCF_AMD_INT4_SYM, DT>(a, sh, s);
+        case NNCF_AMD_NF4: return few_go<NNCF_AMD_NF4, DT>(a, sh, s);
+        default: return few_go<NNCF_AMD_MXFP4, DT>(a, sh, s);
     }
 }
 
-int few_launch(int dtype, int mode, const FewArgs& a, hipStream_t s) {
-    return dtype == NNCF_AMD_BF16 ? few_typed<NNCF_AMD_BF16>(mode, a, s) : few_typed<NNCF_AMD_F16>(mode, a, s);
+int few_launch(int dtype, int mode, const FewArgs& a, const FewShape& sh, hipStream_t s) {
+    return dtype == NNCF_AMD_BF16 ? few_typed<NNCF_AMD_BF16>(mode, a, sh, s) : few_typed<NNCF_AMD_F16>(mode, a, sh, s);
 }
 
 }  // namespace wc

@@ -130,7 +130,7 @@ def _expert_forward(x, w: PackedWeight, slots, offsets, rows: int, top_k: int, g
     z = torch.empty((rows, w.n), dtype=x.dtype, device=x.device) if want_z else None
     L = _lib.lib()
     ws = workspace_of(L.nncf_amd_expert_linear_workspace(_lib.ptr(src), ldx, src.shape[0], int(gather), rows, w.n, w.k, _lib.ptr(w.codes), w.mode,
-                                                         w.group_size, w.experts), x.device)
+                                                         w.group_size, w.experts, act), x.device)
     _lib.check(L.nncf_amd_expert_linear(_lib.ptr(src), _DTYPES[x.dtype], ldx, src.shape[0], _lib.ptr(slots) if gather else None, top_k,
                                         _lib.ptr(offsets), w.experts, rows, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
                                         _lib.ptr(w.scale), _lib.ptr(w.zero_point), act, _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws),

@@ -127,7 +127,7 @@ def activation_grad(dy: torch.Tensor, z: Optional[torch.Tensor], n: int, act: in
         return dy, ldd, None
     L = _lib.lib()
     copies = want_dz and act != 0  # without an activation dz is dy
-    ldz = (n + 31) // 32 * 32
+    ldz = (n + 63) // 64 * 64
     dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
     dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
     ws = workspace_of(L.nncf_amd_activation_grad_workspace(m, n) if want_dbias else 0, dy.device)
@@ -157,7 +157,7 @@ def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_z: b
     res, ldr = (None, 0) if residual is None else rows_of(residual, width)
     L = _lib.lib()
     ws = workspace_of(L.nncf_amd_compressed_linear_workspace(_lib.ptr(rows), ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode,
-                                                             w.group_size), x.device)
+                                                             w.group_size, act), x.device)
     _lib.check(L.nncf_amd_compressed_linear(_lib.ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
                                             _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(bias), act, _lib.ptr(res), ldr,
                                             _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws), 0 if ws is None else ws.numel(),
