@@ -1,5 +1,6 @@
 """ctypes binding of libnncf_amd_wc.so (include/nncf_amd_wc.h).  No fallback: if the library is missing
 the product path raises."""
+import contextlib
 import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
@@ -168,6 +169,20 @@ def ptr(t):
 
 def stream_of(t: torch.Tensor):
     return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(index).cuda_stream holds, without the object
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def raw_stream(t: torch.Tensor) -> int:
+    return _raw_stream(t.get_device())
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which `t`'s device is the current one; costs nothing where it is already."""
+    index = t.get_device()
+    return _SAME_DEVICE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def require_gpu(t: torch.Tensor, what: str) -> None:

@@ -16,7 +16,7 @@ from torch.autograd.function import once_differentiable
 from nncf_amd import _lib
 from nncf_amd import decompressors as dcmp
 from nncf_amd.errors import InternalError
-from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_of, grad_input, packed_weight, rows_of,
+from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_of, grad_input, packed_weight, ptr, rows_of,
                              workspace_of)
 from nncf_amd.parameters import CompressWeightsMode, as_config
 
@@ -40,42 +40,53 @@ class ExpertRouting(NamedTuple):
 
 
 def _route(logits, top_k, renormalize, mask):
+    """(weights, every integer of the routing in one tensor)."""
     tokens, experts = logits.shape
     rows, ldl = rows_of(logits, experts)
-    dev = logits.device
-    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-    ints = torch.empty(3 * tokens * top_k + experts + 1, dtype=torch.int32, device=dev)
-    s = tokens * top_k
-    ids, places, slots, offsets = ints[:s].view(tokens, top_k), ints[s:2 * s].view(tokens, top_k), ints[2 * s:3 * s], ints[3 * s:]
+    slots = tokens * top_k
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=logits.device)
+    ints = torch.empty(3 * slots + experts + 1, dtype=torch.int32, device=logits.device)
+    at = ints.data_ptr()
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_route_experts_workspace(tokens, experts, top_k), dev)
-    _lib.check(L.nncf_amd_route_experts(_lib.ptr(rows), _lib.dtype_id(rows), ldl, tokens, experts, top_k, int(renormalize), _lib.ptr(mask),
-                                        _lib.ptr(weights), _lib.ptr(ids), _lib.ptr(places), _lib.ptr(slots), _lib.ptr(offsets), _lib.ptr(ws),
-                                        0 if ws is None else ws.numel(), _lib.stream_of(logits)))
-    return weights, ids, places, slots, offsets
+    ws = workspace_of(L.nncf_amd_route_experts_workspace(tokens, experts, top_k), logits.device)
+    _lib.check(L.nncf_amd_route_experts(rows.data_ptr(), _lib.dtype_id(rows), ldl, tokens, experts, top_k, int(renormalize), ptr(mask),
+                                        weights.data_ptr(), at, at + 4 * slots, at + 8 * slots, at + 12 * slots, ptr(ws),
+                                        0 if ws is None else ws.numel(), _lib.raw_stream(logits)))
+    return weights, ints
+
+
+def _routing(weights, ints) -> "ExpertRouting":
+    tokens, top_k = weights.shape
+    s = tokens * top_k
+    ids, rows, slots, offsets = ints.split((s, s, s, ints.numel() - 3 * s))
+    return ExpertRouting(weights, ids.view(tokens, top_k), rows.view(tokens, top_k), slots, offsets)
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, renormalize, mask):
-        with torch.cuda.device(logits.device):
-            out = _route(logits, top_k, renormalize, mask)
-        ctx.save_for_backward(logits, out[0], out[1])
+        with _lib.on_device_of(logits):
+            weights, ints = _route(logits, top_k, renormalize, mask)
+        ctx.save_for_backward(logits, weights, ints)
         ctx.renormalize = renormalize
-        ctx.mark_non_differentiable(*out[1:])
-        return out
+        ctx.mark_non_differentiable(ints)
+        ctx.set_materialize_grads(False)
+        return weights, ints
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dweights, *_):
-        logits, weights, ids = ctx.saved_tensors
+    def backward(ctx, dweights, _):
+        if dweights is None:
+            return None, None, None, None
+        logits, weights, ints = ctx.saved_tensors
         tokens, experts = logits.shape
         rows, ldl = rows_of(logits, experts)
+        dweights = dweights.contiguous()
         dlogits = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
-        with torch.cuda.device(logits.device):
+        with _lib.on_device_of(logits):
             _lib.check(_lib.lib().nncf_amd_route_experts_grad(
-                _lib.ptr(rows), _lib.dtype_id(rows), ldl, tokens, experts, ids.shape[1], int(ctx.renormalize), _lib.ptr(weights),
-                _lib.ptr(ids), _lib.ptr(dweights.contiguous()), _lib.ptr(dlogits), _lib.stream_of(logits)))
+                rows.data_ptr(), _lib.dtype_id(rows), ldl, tokens, experts, weights.shape[1], int(ctx.renormalize), weights.data_ptr(),
+                ints.data_ptr(), dweights.data_ptr(), dlogits.data_ptr(), _lib.raw_stream(logits)))
         return dlogits, None, None, None
 
 
@@ -101,24 +112,24 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True, to
             raise InternalError(f"{what}: token_mask is bool [{logits.shape[0]}] on {logits.device}")
         token_mask = token_mask.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return ExpertRouting(*_Route.apply(logits, top_k, bool(renormalize), token_mask))
-    with torch.cuda.device(logits.device):
-        return ExpertRouting(*_route(logits, top_k, renormalize, token_mask))
+        return _routing(*_Route.apply(logits, top_k, bool(renormalize), token_mask))
+    with _lib.on_device_of(logits):
+        return _routing(*_route(logits, top_k, renormalize, token_mask))
 
 
 def _check_routing(routing: ExpertRouting, device, what: str, experts: Optional[int] = None):
     """(tokens, top_k) of a routing whose tensors are as `route_experts` makes them."""
     if not isinstance(routing, ExpertRouting):
         raise InternalError(f"{what}: expected the ExpertRouting of route_experts, got {type(routing).__name__}")
-    tokens, top_k = routing.rows.shape
-    ok = (tuple(routing.weights.shape) == (tokens, top_k) and tuple(routing.slots.shape) == (tokens * top_k,) and routing.offsets.ndim == 1
-          and routing.weights.dtype == torch.float32 and routing.weights.is_contiguous())
-    for t in (routing.rows, routing.slots, routing.offsets):
-        ok = ok and t.dtype == torch.int32 and t.is_contiguous()
-    if not ok:
+    weights, _, rows, slots, offsets = routing
+    tokens, top_k = rows.shape
+    if (weights.shape != rows.shape or slots.shape != (tokens * top_k,) or offsets.ndim != 1 or weights.dtype != torch.float32
+            or rows.dtype != torch.int32 or slots.dtype != torch.int32 or offsets.dtype != torch.int32
+            or not (weights.is_contiguous() and rows.is_contiguous() and slots.is_contiguous() and offsets.is_contiguous())):
         raise InternalError(f"{what}: the routing's tensors are not as route_experts makes them")
-    if any(t.device != device for t in (routing.weights, routing.rows, routing.slots, routing.offsets)):
-        raise InternalError(f"{what}: the routing is on {routing.rows.device}, the activations on {device}")
+    index = device.index
+    if rows.get_device() != index or weights.get_device() != index or slots.get_device() != index or offsets.get_device() != index:
+        raise InternalError(f"{what}: the routing is on {rows.device}, the activations on {device}")
     if experts is not None and routing.offsets.numel() != experts + 1:
         raise InternalError(f"{what}: a routing over {routing.offsets.numel() - 1} experts for a stack of {experts}")
     return tokens, top_k
@@ -129,19 +140,19 @@ def _expert_forward(x, w: PackedWeight, slots, offsets, rows: int, top_k: int, g
     y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
     z = torch.empty((rows, w.n), dtype=x.dtype, device=x.device) if want_z else None
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_expert_linear_workspace(_lib.ptr(src), ldx, src.shape[0], int(gather), rows, w.n, w.k, _lib.ptr(w.codes), w.mode,
+    ws = workspace_of(L.nncf_amd_expert_linear_workspace(ptr(src), ldx, src.shape[0], int(gather), rows, w.n, w.k, ptr(w.codes), w.mode,
                                                          w.group_size, w.experts, act), x.device)
-    _lib.check(L.nncf_amd_expert_linear(_lib.ptr(src), _DTYPES[x.dtype], ldx, src.shape[0], _lib.ptr(slots) if gather else None, top_k,
-                                        _lib.ptr(offsets), w.experts, rows, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
-                                        _lib.ptr(w.scale), _lib.ptr(w.zero_point), act, _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws),
-                                        0 if ws is None else ws.numel(), _lib.stream_of(x)))
+    _lib.check(L.nncf_amd_expert_linear(ptr(src), _DTYPES[x.dtype], ldx, src.shape[0], ptr(slots) if gather else None, top_k,
+                                        ptr(offsets), w.experts, rows, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
+                                        ptr(w.scale), ptr(w.zero_point), act, ptr(y), width, ptr(z), ptr(ws),
+                                        0 if ws is None else ws.numel(), _lib.raw_stream(x)))
     return y, z
 
 
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, slots, offsets, places, gather, act, width):
-        with torch.cuda.device(x.device):
+        with _lib.on_device_of(x):
             y, z = _expert_forward(x, w, slots, offsets, slots.shape[0], places.shape[1], gather, act, width, act != 0)
         ctx.save_for_backward(z, w.codes, w.scale, w.zero_point, offsets, places)
         ctx.weight, ctx.act, ctx.dtype, ctx.gather = w[3:], act, x.dtype, gather
@@ -152,7 +163,7 @@ class _ExpertLinear(torch.autograd.Function):
     def backward(ctx, dy):
         z, codes, scale, zp, offsets, places = ctx.saved_tensors
         w = PackedWeight(codes, scale, zp, *ctx.weight)
-        with torch.cuda.device(dy.device):
+        with _lib.on_device_of(dy):
             dz, ldz, _ = activation_grad(dy, z, w.n, ctx.act, ctx.dtype, True, False)
             # a token's rows are added up in fp32 and rounded once
             dx = grad_input(dz, ldz, w, offsets, ctx.dtype, fp32=ctx.gather)
@@ -180,7 +191,7 @@ def expert_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, routing: 
         raise InternalError(f"{what}: x of shape {tuple(x.shape)}, expected {(tokens if gather else rows, w.k)}")
     if torch.is_grad_enabled() and x.requires_grad:
         return _ExpertLinear.apply(x, w, routing.slots, routing.offsets, routing.rows, bool(gather), act, width)
-    with torch.cuda.device(x.device):
+    with _lib.on_device_of(x):
         return _expert_forward(x, w, routing.slots, routing.offsets, rows, top_k, bool(gather), act, width, False)[0]
 
 
@@ -189,15 +200,15 @@ def _combine(y, weights, places, dtype):
     n = y.shape[1]
     src, ldy = rows_of(y, n) if n else (y, 0)
     out = torch.empty((tokens, n), dtype=dtype, device=y.device)
-    _lib.check(_lib.lib().nncf_amd_combine_experts(_lib.ptr(src), _lib.dtype_id(src), ldy, src.shape[0], _lib.ptr(weights), _lib.ptr(places),
-                                                   tokens, top_k, n, _lib.ptr(out), _DTYPES[dtype], _lib.stream_of(y)))
+    _lib.check(_lib.lib().nncf_amd_combine_experts(ptr(src), _lib.dtype_id(src), ldy, src.shape[0], ptr(weights), ptr(places),
+                                                   tokens, top_k, n, ptr(out), _DTYPES[dtype], _lib.raw_stream(y)))
     return out
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, places, slots):
-        with torch.cuda.device(y.device):
+        with _lib.on_device_of(y):
             out = _combine(y, weights, places, y.dtype)
         ctx.save_for_backward(y, weights, places, slots)
         return out
@@ -213,10 +224,10 @@ class _Combine(torch.autograd.Function):
         dy = torch.empty(y.shape, dtype=y.dtype, device=y.device) if need_y else None
         dw = torch.empty((tokens, top_k), dtype=torch.float32, device=y.device) if need_w else None
         dout = dout.contiguous()
-        with torch.cuda.device(y.device):
+        with _lib.on_device_of(y):
             _lib.check(_lib.lib().nncf_amd_combine_experts_grad(
-                _lib.ptr(dout), _DTYPES[y.dtype], _lib.ptr(src), ldy, _lib.ptr(weights), _lib.ptr(places), _lib.ptr(slots), tokens, top_k, n,
-                _lib.ptr(dy), _lib.ptr(dw), _lib.stream_of(y)))
+                ptr(dout), _DTYPES[y.dtype], ptr(src), ldy, ptr(weights), ptr(places), ptr(slots), tokens, top_k, n,
+                ptr(dy), ptr(dw), _lib.raw_stream(y)))
         return dy, dw, None, None
 
 
@@ -232,7 +243,7 @@ def combine_experts(y: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
         raise InternalError(f"{what}: y of shape {tuple(y.shape)} for {tokens * top_k} rows")
     if torch.is_grad_enabled() and (y.requires_grad or routing.weights.requires_grad):
         return _Combine.apply(y, routing.weights, routing.rows, routing.slots)
-    with torch.cuda.device(y.device):
+    with _lib.on_device_of(y):
         return _combine(y, routing.weights, routing.rows, y.dtype)
 
 

@@ -10,6 +10,7 @@ sums are fp32 and the result is rounded once.
 """
 from __future__ import annotations
 
+import math
 import types
 from typing import NamedTuple, Optional, Tuple
 
@@ -39,14 +40,19 @@ class PackedWeight(NamedTuple):
     group_size: int
 
 
+_MODE_OF = {dcmp.INT8AsymmetricWeightsDecompressor: "int8_asym", dcmp.INT8SymmetricWeightsDecompressor: "int8_sym",
+            dcmp.INT4AsymmetricWeightsDecompressor: "int4_asym", dcmp.INT4SymmetricWeightsDecompressor: "int4_sym",
+            dcmp.NF4WeightsDecompressor: "nf4", dcmp.MXFP4WeightsDecompressor: "mxfp4"}
+
+
 def _mode_of(decompressor) -> str:
-    if isinstance(decompressor, dcmp._FourBit):
-        return decompressor._mode
-    if isinstance(decompressor, dcmp.INT8AsymmetricWeightsDecompressor):
-        return "int8_asym"
-    if isinstance(decompressor, dcmp.INT8SymmetricWeightsDecompressor):
-        return "int8_sym"
-    raise InternalError(f"{type(decompressor).__name__} is not a decompressor of this package")
+    mode = _MODE_OF.get(type(decompressor))
+    if mode is None:
+        for cls, mode in _MODE_OF.items():
+            if isinstance(decompressor, cls):
+                return mode
+        raise InternalError(f"{type(decompressor).__name__} is not a decompressor of this package")
+    return mode
 
 
 def weight_dtype_of(decompressor) -> torch.dtype:
@@ -59,39 +65,41 @@ def weight_dtype_of(decompressor) -> torch.dtype:
 def packed_weight(packed: torch.Tensor, decompressor, x: torch.Tensor, ndim: int, what: str) -> PackedWeight:
     """`packed` and its decompressor as the kernels take them; ndim: 2 for [n, k], 3 for [experts, n, k]."""
     mode = _mode_of(decompressor)
-    if x.dtype not in _DTYPES:
-        raise InternalError(f"{what}: activations are float16 or bfloat16, got {x.dtype}")
-    if weight_dtype_of(decompressor) != x.dtype:
-        raise InternalError(f"{what}: activations are {x.dtype}, the decompressed weight is {weight_dtype_of(decompressor)}")
-    scale = decompressor._scale
-    four = isinstance(decompressor, dcmp._FourBit)
+    dtype, device = x.dtype, x.get_device()
+    if dtype not in _DTYPES:
+        raise InternalError(f"{what}: activations are float16 or bfloat16, got {dtype}")
+    if weight_dtype_of(decompressor) != dtype:
+        raise InternalError(f"{what}: activations are {dtype}, the decompressed weight is {weight_dtype_of(decompressor)}")
+    buffers = decompressor._buffers  # (module attributes are looked up through several dictionaries)
+    scale, zp = buffers["_scale"], buffers.get("_zero_point")
+    four = mode not in ("int8_sym", "int8_asym")
     if four:
         grouped = tuple(decompressor.compressed_weight_shape)
         shape = grouped if decompressor.result_shape is None else tuple(decompressor.result_shape)
     else:
         shape = grouped = tuple(packed.shape)
-    if len(shape) != ndim or 0 in shape:
+    elements, n_groups = math.prod(shape), scale.numel()
+    if len(shape) != ndim or elements == 0:
         raise InternalError(f"{what}: the weight is {ndim}-dimensional and not empty, got shape {shape}")
-    n_groups, group_size = dcmp._groups(grouped, scale)
-    experts, (n, k) = (1 if ndim == 2 else shape[0]), shape[-2:]
-    if n_groups * group_size != experts * n * k or k % group_size:
-        raise InternalError(f"{what}: groups of {group_size} do not divide rows of {k} (weight {shape}, scale {tuple(scale.shape)})")
-    codes = packed.detach()
-    if codes.dtype != (torch.int8 if mode == "int8_sym" else torch.uint8):
-        raise InternalError(f"{what}: packed codes of type {codes.dtype} for mode {mode}")
-    if codes.numel() != (experts * n * k // 2 if four else experts * n * k):
-        raise InternalError(f"{what}: {codes.numel()} bytes of codes for a weight of shape {shape}, mode {mode}")
+    n, k = shape[-2:]
+    group_size = elements // n_groups if n_groups else 0
+    if tuple(scale.shape) != grouped[:-1] + (1,) or group_size * n_groups != elements or k % group_size:
+        raise InternalError(f"{what}: scales {tuple(scale.shape)} do not divide a weight of shape {shape} ({grouped}) into groups")
+    if packed.dtype != (torch.int8 if mode == "int8_sym" else torch.uint8):
+        raise InternalError(f"{what}: packed codes of type {packed.dtype} for mode {mode}")
+    if packed.numel() != (elements // 2 if four else elements):
+        raise InternalError(f"{what}: {packed.numel()} bytes of codes for a weight of shape {shape}, mode {mode}")
     if scale.dtype != (torch.uint8 if mode == "mxfp4" else torch.float16):
         raise InternalError(f"{what}: scales of type {scale.dtype} for mode {mode}")
-    zp = getattr(decompressor, "_zero_point", None)
-    for t in (codes, scale, zp):
-        if t is not None and t.device != x.device:
-            raise InternalError(f"{what}: the weight is on {t.device}, the activations on {x.device}")
+    if packed.get_device() != device or scale.get_device() != device or (zp is not None and zp.get_device() != device):
+        raise InternalError(f"{what}: the weight is on {packed.device} and {scale.device}, the activations on {x.device}")
     if zp is not None:
         if zp.dtype != torch.uint8 or zp.numel() != ((n_groups + 1) // 2 if four else n_groups):
             raise InternalError(f"{what}: {zp.numel()} bytes of zero points ({zp.dtype}) for {n_groups} groups, mode {mode}")
-        zp = zp.contiguous()
-    return PackedWeight(codes.contiguous(), scale.contiguous(), zp, _lib.MODE_ID[mode], experts, n, k, group_size)
+        if not zp.is_contiguous():
+            zp = zp.contiguous()
+    return PackedWeight(packed if packed.is_contiguous() else packed.contiguous(), scale if scale.is_contiguous() else scale.contiguous(), zp,
+                        _lib.MODE_ID[mode], shape[0] if ndim == 3 else 1, n, k, group_size)
 
 
 def activation_of(activation: Optional[str], n: int, what: str) -> Tuple[int, int]:
@@ -108,10 +116,17 @@ def activation_of(activation: Optional[str], n: int, what: str) -> Tuple[int, in
 
 def rows_of(t: torch.Tensor, width: int) -> Tuple[torch.Tensor, int]:
     """`t` [..., width] as rows of consecutive elements and their distance (copied where its strides do not allow it)."""
-    t = t.reshape(-1, width)
+    if t.ndim != 2:
+        t = t.reshape(-1, width)
+    if t.is_contiguous():
+        return t, width
     if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
-        t = t.contiguous()
+        return t.contiguous(), width
     return t, t.stride(0) if t.shape[0] > 1 else width
+
+
+def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def workspace_of(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -131,8 +146,8 @@ def activation_grad(dy: torch.Tensor, z: Optional[torch.Tensor], n: int, act: in
     dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
     dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
     ws = workspace_of(L.nncf_amd_activation_grad_workspace(m, n) if want_dbias else 0, dy.device)
-    _lib.check(L.nncf_amd_activation_grad(_lib.ptr(dy), _DTYPES[dtype], ldd, _lib.ptr(z), m, n, act, _lib.ptr(dz), ldz, _lib.ptr(dbias),
-                                          _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(dy)))
+    _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(z), m, n, act, ptr(dz), ldz, ptr(dbias),
+                                          ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dy)))
     return (dz, ldz, dbias) if copies else (dy, ldd, dbias)
 
 
@@ -141,10 +156,10 @@ def grad_input(dz: torch.Tensor, ldz: int, w: PackedWeight, offsets: Optional[to
     L = _lib.lib()
     m = dz.shape[0]
     dx = torch.empty((m, w.k), dtype=torch.float32 if fp32 else dtype, device=dz.device)
-    ws = workspace_of(L.nncf_amd_linear_grad_input_workspace(_lib.ptr(dz), ldz, m, w.n, w.k, w.experts), dz.device)
-    _lib.check(L.nncf_amd_linear_grad_input(_lib.ptr(dz), _DTYPES[dtype], ldz, _lib.ptr(offsets), w.experts, m, w.n, w.k, _lib.ptr(w.codes),
-                                            w.mode, w.group_size, _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(dx), w.k, int(fp32),
-                                            _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_of(dz)))
+    ws = workspace_of(L.nncf_amd_linear_grad_input_workspace(ptr(dz), ldz, m, w.n, w.k, w.experts), dz.device)
+    _lib.check(L.nncf_amd_linear_grad_input(ptr(dz), _DTYPES[dtype], ldz, ptr(offsets), w.experts, m, w.n, w.k, ptr(w.codes),
+                                            w.mode, w.group_size, ptr(w.scale), ptr(w.zero_point), ptr(dx), w.k, int(fp32),
+                                            ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dz)))
     return dx
 
 
@@ -156,19 +171,19 @@ def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_z: b
     z = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if want_z else None
     res, ldr = (None, 0) if residual is None else rows_of(residual, width)
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(_lib.ptr(rows), ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode,
+    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(ptr(rows), ldx, m, w.n, w.k, ptr(w.codes), w.mode,
                                                              w.group_size, act), x.device)
-    _lib.check(L.nncf_amd_compressed_linear(_lib.ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, _lib.ptr(w.codes), w.mode, w.group_size,
-                                            _lib.ptr(w.scale), _lib.ptr(w.zero_point), _lib.ptr(bias), act, _lib.ptr(res), ldr,
-                                            _lib.ptr(y), width, _lib.ptr(z), _lib.ptr(ws), 0 if ws is None else ws.numel(),
-                                            _lib.stream_of(x)))
+    _lib.check(L.nncf_amd_compressed_linear(ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
+                                            ptr(w.scale), ptr(w.zero_point), ptr(bias), act, ptr(res), ldr,
+                                            ptr(y), width, ptr(z), ptr(ws), 0 if ws is None else ws.numel(),
+                                            _lib.raw_stream(x)))
     return y, z
 
 
 class _CompressedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w, act, width):
-        with torch.cuda.device(x.device):
+        with _lib.on_device_of(x):
             y, z = _forward(x, w, bias, act, width, residual, act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]))
         ctx.save_for_backward(z, w.codes, w.scale, w.zero_point)
         ctx.weight, ctx.act, ctx.shape, ctx.dtype = w[3:], act, x.shape, x.dtype
@@ -182,7 +197,7 @@ class _CompressedLinear(torch.autograd.Function):
         need_x, need_bias, need_residual = ctx.needs_input_grad[:3]
         dx = dbias = None
         if need_x or need_bias:
-            with torch.cuda.device(dy.device):
+            with _lib.on_device_of(dy):
                 dz, ldz, dbias = activation_grad(dy, z, w.n, ctx.act, ctx.dtype, need_x, need_bias)
                 if need_x:
                     dx = grad_input(dz, ldz, w, None, ctx.dtype).reshape(ctx.shape)
@@ -217,11 +232,12 @@ def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias:
                                 f"{tuple(x.shape[:-1]) + (width,)} {x.dtype} on {x.device}")
     if bias is not None and not bias.is_contiguous():
         bias = bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
         return _CompressedLinear.apply(x, bias, residual, w, act, width)
-    with torch.cuda.device(x.device):
+    with _lib.on_device_of(x):
         y, _ = _forward(x, w, bias, act, width, residual, False)
-    return y.reshape(x.shape[:-1] + (width,))
+    return y if x.ndim == 2 else y.reshape(x.shape[:-1] + (width,))
 
 
 # ------------------------------------------------------------------------------------------------------------- models
