@@ -15,7 +15,7 @@ constexpr int kRouteWaves = kRouteThreads / 64;
 constexpr int kRouteSlots = 4096;      // slots of one block: their experts and ranks are held in LDS
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopk = 64;
-constexpr int kRouteBlocks = 128;      // blocks that the tokens are dealt over while the slots of a block fit
+constexpr int kRouteBlocks = 256;      // blocks that the tokens are dealt over while the slots of a block fit
 
 template <int DT>
 __device__ __forceinline__ float logit(const void* p, int64_t i) { return Elem<DT>::load(p, i); }
@@ -32,6 +32,25 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 }
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
     return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)v, d, 64);
+}
+
+// maximum over aligned sets of G lanes: inside 16 lanes by DPP (a shuffle goes through LDS), above that by shuffles
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp64(uint64_t v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, true);
+    return (uint64_t)hi << 32 | lo;
+}
+template <int G>
+__device__ __forceinline__ uint64_t max_over(uint64_t v) {
+    auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+    if constexpr (G >= 2) v = larger(v, dpp64<0xB1>(v));    // quad_perm [1,0,3,2]
+    if constexpr (G >= 4) v = larger(v, dpp64<0x4E>(v));    // quad_perm [2,3,0,1]
+    if constexpr (G >= 8) v = larger(v, dpp64<0x141>(v));   // row_half_mirror
+    if constexpr (G >= 16) v = larger(v, dpp64<0x140>(v));  // row_mirror
+    if constexpr (G >= 32) v = larger(v, shfl_xor64(v, 16));
+    if constexpr (G >= 64) v = larger(v, shfl_xor64(v, 32));
+    return v;
 }
 
 struct RouteArgs {
@@ -82,11 +101,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
             uint64_t best = key[0];
 #pragma unroll
             for (int i = 1; i < V; ++i) best = key[i] > best ? key[i] : best;
-#pragma unroll
-            for (int d = 1; d < G; d <<= 1) {
-                const uint64_t o = shfl_xor64(best, d);
-                best = o > best ? o : best;
-            }
+            best = max_over<G>(best);
             const float v = value_of((uint32_t)(best >> 32));
             if (j == 0) {
                 top = v;
@@ -94,8 +109,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
 #pragma unroll
                     for (int i = 0; i < V; ++i)
                         if (key[i]) all += expf(value_of((uint32_t)(key[i] >> 32)) - top);
-#pragma unroll
-                    for (int d = 1; d < G; d <<= 1) all += __shfl_xor(all, d, 64);
+                    all = lanes_allreduce<G>(all, OpAdd());
                 }
             }
 #pragma unroll
@@ -109,9 +123,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs a) {
                 a.ids[t * a.topk + j] = masked ? -1 : e;
             }
         }
-        int any_nan = nan;
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) any_nan |= __shfl_xor(any_nan, d, 64);
+        const bool any_nan = max_over<G>(nan) != 0;
         if (gl == 0 && live) {
             const float total = a.renormalize ? chosen : all;
             const bool none = masked || (top == -__builtin_inff() && !any_nan);
@@ -260,16 +272,14 @@ __global__ __launch_bounds__(256) void k_route_grad(const void* __restrict__ log
             x[i] = e < experts ? logit<DT>(logits, tt * ldl + e) : -__builtin_inff();
             top = fmaxf(top, x[i]);
         }
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        top = lanes_allreduce<G>(top, OpMax());
         const bool empty = top == -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             p[i] = i * G + gl < experts && !empty ? expf(x[i] - top) : 0.0f;
             all += p[i];
         }
-#pragma unroll
-        for (int d = 1; d < G; d <<= 1) all += __shfl_xor(all, d, 64);
+        all = lanes_allreduce<G>(all, OpAdd());
         if (empty) all = 1.0f;
     }
     for (int j = 0; j < topk; ++j) dot += weights[tt * topk + j] * dweights[tt * topk + j];

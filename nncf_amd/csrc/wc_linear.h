@@ -158,10 +158,24 @@ __device__ __forceinline__ void fill_nf4(h2* lut) {
 __device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 constexpr float kGeluC = 1.5957691216057308f;  // 2 * sqrt(2 / pi): tanh(u) written as 2 * sigmoid(2 u) - 1
 
+// Phi(z), the normal distribution's integral, by Abramowitz and Stegun 7.1.26: erfc(x) = t (a1 + ... + a5 t^4) e^(-x^2) with
+// t = 1 / (1 + 0.3275911 x), x = |z| / sqrt(2), off by at most 1.5e-7; as a factor of e^(-x^2) it keeps the small values of the
+// left tail.  (The library's erfcf takes about 100 instructions: 20 us of the epilogue of 2047 x 4096 results.)
+__device__ __forceinline__ float normal_cdf(float z) {
+    const float x = 0.70710678118654752f * fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+    float p = 1.061405429f;
+    p = __builtin_fmaf(p, t, -1.453152027f);
+    p = __builtin_fmaf(p, t, 1.421413741f);
+    p = __builtin_fmaf(p, t, -0.284496736f);
+    p = __builtin_fmaf(p, t, 0.254829592f);
+    const float tail = 0.5f * p * t * __expf(-x * x);
+    return z > 0.0f ? 1.0f - tail : tail;
+}
+
 __device__ __forceinline__ float activate(int act, float z) {
     switch (act) {
         case kActRelu: return z > 0.0f ? z : (z == z ? 0.0f : z);
-        case kActGelu: return 0.5f * z * erfcf(-0.70710678118654752f * z);  // erfc keeps the small values of the left tail
+        case kActGelu: return z * normal_cdf(z);
         case kActGeluTanh: return z * sigmoid_f(kGeluC * (z + 0.044715f * z * z * z));
         case kActSilu: return z * sigmoid_f(z);
         default: return z;
@@ -172,7 +186,7 @@ __device__ __forceinline__ float activate_grad(int act, float z) {
     z = z > 1e4f ? 1e4f : (z < -1e4f ? -1e4f : z);
     switch (act) {
         case kActRelu: return z > 0.0f ? 1.0f : 0.0f;
-        case kActGelu: return 0.5f * erfcf(-0.70710678118654752f * z) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        case kActGelu: return normal_cdf(z) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
         case kActGeluTanh: {
             const float s = sigmoid_f(kGeluC * (z + 0.044715f * z * z * z));
             return s + z * s * (1.0f - s) * kGeluC * (1.0f + 0.134145f * z * z);

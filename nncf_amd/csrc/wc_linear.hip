@@ -11,40 +11,59 @@ namespace wc {
 constexpr int64_t round64(int64_t v) { return (v + 63) / 64 * 64; }
 
 // ---------------------------------------------------------------------------------- weight -> dense rows of the workspace
-// [experts * n, kp], kp = k rounded up to 64, the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  A block
-// takes ROWS rows; a thread 8 consecutive weights of a row, whose place and group come from multiplications by 2^32 / d
-// (exact while the product of both factors is below 2^32: k up to 131072).  An expert without rows is left out.
-constexpr int kDequantRows = 8;
+// [experts * n, kp], kp = k rounded up to 64, the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  `lanes` (a
+// power of two) threads follow a row, 8 weights each; a thread takes the same place of kDequantRows rows, whose reads are
+// requested together and whose addresses are a scalar apart.  An expert without rows is left out.
+constexpr int kDequantRows = 4;
 template <int MODE, int DT>
 __global__ __launch_bounds__(256) void k_dequant_rows(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
                                                       const uint8_t* __restrict__ zp, uint16_t* __restrict__ out, int64_t total_rows,
-                                                      int64_t n, uint32_t k, uint32_t kp, uint32_t groups, uint32_t magic_row,
-                                                      uint32_t magic_group, const RowMap rows) {
+                                                      int64_t n, uint32_t k, uint32_t kp, uint32_t groups, uint32_t magic_group, int log_lanes,
+                                                      const RowMap rows) {
     __shared__ h2 lut[MODE == NNCF_AMD_NF4 ? kNf4Pairs : 1];
     fill_nf4<MODE>(lut);
-    const int64_t row0 = (int64_t)blockIdx.x * kDequantRows;
-    const uint32_t vecs = kp / 8;
-    for (uint32_t i = threadIdx.x; i < kDequantRows * vecs; i += 256) {
-        const uint32_t r = __umulhi(i, magic_row), v = i - r * vecs;
-        const int64_t row = row0 + r;
-        if (row >= total_rows) break;
-        if (rows.offsets) {
+    const uint32_t lanes = 1u << log_lanes, strips = 256u >> log_lanes;  // strips of kDequantRows rows
+    const int64_t block0 = (int64_t)blockIdx.x * strips * kDequantRows;
+    if (rows.offsets) {  // (a block that reaches into an expert with rows takes all of its rows)
+        const int64_t block1 = block0 + strips * kDequantRows < total_rows ? block0 + strips * kDequantRows : total_rows;
+        bool any = false;
+        for (int64_t e = block0 / n; e <= (block1 - 1) / n; ++e) {
             int64_t lo, hi;
-            expert_range(rows, (int)(row / n), lo, hi);
-            if (lo >= hi) continue;
+            expert_range(rows, (int)e, lo, hi);
+            any = any || lo < hi;
         }
-        u32v4 w{0, 0, 0, 0};
-        if (v * 8 < k) {
-            const GroupPar<MODE> g = group_par<MODE>(scale, zp, row * groups + __umulhi(v, magic_group));
-            const int64_t e0 = row * k + v * 8;
-            if constexpr (four_bit(MODE)) {
-                w = dequant8<MODE, DT>(*(const uint32_t*)(codes + e0 / 2), 0, g, lut);
-            } else {
-                const u32v2 p = *(const u32v2*)(codes + e0);
-                w = dequant8<MODE, DT>(p.x, p.y, g, lut);
-            }
+        if (!any) return;
+    }
+    const uint32_t row_bytes = four_bit(MODE) ? k / 2 : k;
+    const uint32_t strip = threadIdx.x >> log_lanes;
+    const int64_t row0 = block0 + strip * kDequantRows;
+    if (row0 >= total_rows) return;
+    const int here = total_rows - row0 < kDequantRows ? (int)(total_rows - row0) : kDequantRows;
+    const uint8_t* c0 = codes + row0 * row_bytes;
+    const int64_t g0 = row0 * groups;
+    uint16_t* o0 = out + row0 * kp;
+    for (uint32_t v = threadIdx.x & (lanes - 1); v < kp / 8; v += lanes) {
+        if (v * 8 >= k) {
+            for (int r = 0; r < here; ++r) *(u32v4*)(o0 + (uint64_t)r * kp + v * 8) = u32v4{0, 0, 0, 0};
+            continue;
         }
-        *(u32v4*)(out + row * kp + v * 8) = w;
+        const uint32_t g = magic_group ? __umulhi(v, magic_group) : v;
+        u32v2 p[kDequantRows];
+        uint32_t sc[kDequantRows], zr[kDequantRows];
+#pragma unroll
+        for (int r = 0; r < kDequantRows; ++r) {
+            const uint32_t rr = r < here ? r : 0;
+            if constexpr (four_bit(MODE)) p[r].x = *(const uint32_t*)(c0 + (uint64_t)rr * row_bytes + v * 4);
+            else p[r] = *(const u32v2*)(c0 + (uint64_t)rr * row_bytes + v * 8);
+            const int64_t gi = g0 + rr * groups + g;
+            if constexpr (MODE == NNCF_AMD_MXFP4) sc[r] = ((const uint8_t*)scale)[gi];
+            else sc[r] = ((const uint16_t*)scale)[gi];
+            if constexpr (MODE == NNCF_AMD_INT4_ASYM) zr[r] = (uint32_t)(zp[gi >> 1] >> (4 * (gi & 1))) & 15u;
+            if constexpr (MODE == NNCF_AMD_INT8_ASYM) zr[r] = zp[gi];
+        }
+#pragma unroll
+        for (int r = 0; r < kDequantRows; ++r)
+            if (r < here) *(u32v4*)(o0 + (uint64_t)r * kp + v * 8) = dequant8<MODE, DT>(p[r].x, p[r].y, par_of<MODE>(sc[r], zr[r]), lut);
     }
 }
 
@@ -69,14 +88,15 @@ __global__ __launch_bounds__(256) void k_dequant_rows_any(const uint8_t* __restr
 }
 
 // ------------------------------------------------------------------------- weight -> its transpose, for the gradient of x
-// [experts, k, np], np = n rounded up to 64, the tail zero: tiles of 64 x 64 turned round in LDS (rows padded by 4 bytes so
-// that the columns that are written fall on different banks).
+// [experts, k, np], np = n rounded up to 64, the tail zero: tiles of 64 x 64 turned round in LDS as pairs of neighbouring n
+// (rows padded by 4 bytes so that the columns that are written fall on different banks).
+constexpr int kTurns = 4;
 template <int MODE, int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_dequant_transposed(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
                                                             const uint8_t* __restrict__ zp, uint16_t* __restrict__ out, int64_t n,
                                                             int64_t k, int64_t np, int64_t gs, const RowMap rows) {
     __shared__ h2 lut[MODE == NNCF_AMD_NF4 ? kNf4Pairs : 1];
-    __shared__ uint16_t tile[64][66];  // [k][n]
+    __shared__ uint32_t tile[64][33];  // [k][pairs of n]
     fill_nf4<MODE>(lut);
     const int expert = blockIdx.z;
     if (rows.offsets) {
@@ -84,42 +104,61 @@ __global__ __launch_bounds__(256) void k_dequant_transposed(const uint8_t* __res
         expert_range(rows, expert, lo, hi);
         if (lo >= hi) return;
     }
-    const int64_t n0 = (int64_t)blockIdx.x * 64, k0 = (int64_t)blockIdx.y * 64, groups = k / gs;
-    for (int i = threadIdx.x; i < 512; i += 256) {  // 64 rows x 8 vectors of 8 k
-        const int nr = i >> 3, v = (i & 7) * 8;
-        const int64_t row = n0 + nr, c = k0 + v;
-        uint16_t w[8] = {};
-        if (row < n) {
-            const int64_t e0 = ((int64_t)expert * n + row) * k + c;
+    // kTurns tiles one behind the other along k: their reads, 32 or 64 bytes of a row each, are requested together
+    const int64_t n0 = (int64_t)blockIdx.x * 64, kb = (int64_t)blockIdx.y * 64 * kTurns, groups = k / gs;
+    const int pair = threadIdx.x >> 3, v = (threadIdx.x & 7) * 8;  // a thread: two rows of W, 8 k of each
+    u32v2 p[kTurns][2];
+    uint32_t sc[kTurns][2], zr[kTurns][2];
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                int64_t row = n0 + 2 * pair + h, c = kb + 64 * t + v;  // (rows and k behind the end: any, their place gets zeros)
+                row = row < n ? row : n - 1;
+                c = c < k ? c : 0;
+                const int64_t at = (int64_t)expert * n + row, e0 = at * k + c, g = at * groups + (uint32_t)c / (uint32_t)gs;
+                if constexpr (four_bit(MODE)) p[t][h].x = *(const uint32_t*)(codes + e0 / 2);
+                else p[t][h] = *(const u32v2*)(codes + e0);
+                if constexpr (MODE == NNCF_AMD_MXFP4) sc[t][h] = ((const uint8_t*)scale)[g];
+                else sc[t][h] = ((const uint16_t*)scale)[g];
+                if constexpr (MODE == NNCF_AMD_INT4_ASYM) zr[t][h] = (uint32_t)(zp[g >> 1] >> (4 * (g & 1))) & 15u;
+                if constexpr (MODE == NNCF_AMD_INT8_ASYM) zr[t][h] = zp[g];
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t) {
+        const int64_t k0 = kb + 64 * t;
+        if (k0 >= k) break;
+        uint16_t w[2][8] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t row = n0 + 2 * pair + h, c = k0 + v;
+            if (row >= n) continue;
             if constexpr (ALIGNED) {
                 if (c < k) {
-                    const GroupPar<MODE> g = group_par<MODE>(scale, zp, ((int64_t)expert * n + row) * groups + c / gs);
-                    u32v4 o;
-                    if constexpr (four_bit(MODE)) o = dequant8<MODE, DT>(*(const uint32_t*)(codes + e0 / 2), 0, g, lut);
-                    else {
-                        const u32v2 p = *(const u32v2*)(codes + e0);
-                        o = dequant8<MODE, DT>(p.x, p.y, g, lut);
-                    }
+                    const u32v4 o = dequant8<MODE, DT>(p[t][h].x, p[t][h].y, par_of<MODE>(sc[t][h], zr[t][h]), lut);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) w[2 * j] = (uint16_t)o[j], w[2 * j + 1] = (uint16_t)(o[j] >> 16);
+                    for (int j = 0; j < 4; ++j) w[h][2 * j] = (uint16_t)o[j], w[h][2 * j + 1] = (uint16_t)(o[j] >> 16);
                 }
             } else {
+                const int64_t e0 = ((int64_t)expert * n + row) * k + c;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (c + j < k) w[j] = dequant1<MODE, DT>(codes, e0 + j, group_par<MODE>(scale, zp, (e0 + j) / gs), lut);
+                    if (c + j < k) w[h][j] = dequant1<MODE, DT>(codes, e0 + j, group_par<MODE>(scale, zp, (e0 + j) / gs), lut);
             }
         }
+        if (t > 0) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) tile[v + j][nr] = w[j];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 512; i += 256) {  // 64 rows of k x 8 vectors of 8 n
-        const int kr = i >> 3, v = (i & 7) * 8;
-        if (k0 + kr >= k || n0 + v >= np) continue;
-        u32v4 o;
+        for (int j = 0; j < 8; ++j) tile[v + j][pair] = w[0][j] | (uint32_t)w[1][j] << 16;
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = *(const uint32_t*)&tile[kr][v + 2 * j];
-        *(u32v4*)(out + ((int64_t)expert * k + k0 + kr) * np + n0 + v) = o;
+        for (int u = 0; u < 2; ++u) {  // 64 rows of k x 8 vectors of 8 n
+            const int kr = pair + 32 * u, nv = (threadIdx.x & 7) * 4;
+            if (k0 + kr < k && n0 + 2 * nv < np)
+                *(u32v4*)(out + ((int64_t)expert * k + k0 + kr) * np + n0 + 2 * nv) =
+                    u32v4{tile[kr][nv], tile[kr][nv + 1], tile[kr][nv + 2], tile[kr][nv + 3]};
+        }
     }
 }
 
@@ -135,49 +174,100 @@ __global__ __launch_bounds__(256) void k_pack_rows(const uint16_t* __restrict__ 
 // dz = dy * act'(z) (swiglu: both halves), written with row stride ldz and zeros behind n; and the sums of dz's fp32 values
 // over chunks of 32 rows, which k_sum_chunks adds up in order (no atomics: the result does not depend on the schedule).
 // dz is rounded to the activations' type because the product that takes it reads 16-bit operands.
+// A thread takes VEC consecutive columns; the chunk's rows are dealt to 4 waves whose sums meet in LDS, wave 0 first.
 constexpr int kChunkRows = 32;
-template <int DT>
+template <int DT, int VEC>
 __global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restrict__ dy, int64_t ldd, const uint16_t* __restrict__ z,
                                                          int64_t m, int64_t n, int act, uint16_t* __restrict__ dz, int64_t ldz,
                                                          float* __restrict__ sums) {
+    __shared__ float part[3][2 * VEC][64];
     const int64_t width = act == kActSwiglu ? n / 2 : n;
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * VEC;
     const int64_t r0 = (int64_t)blockIdx.y * kChunkRows, r1 = r0 + kChunkRows < m ? r0 + kChunkRows : m;
-    if (c >= width) {
-        const int64_t pad = n + (c - width);  // the padding's columns, by the threads behind the last column
-        if (dz && pad < ldz)
-            for (int64_t r = r0; r < r1; ++r) dz[r * ldz + pad] = 0;
-        return;
-    }
-    float s0 = 0.0f, s1 = 0.0f;
-    for (int64_t r = r0; r < r1; ++r) {
-        const float g = to_f32<DT>(dy[r * ldd + c]);
-        float a = g;
-        if (act == kActSwiglu) {
-            const float zg = to_f32<DT>(z[r * n + c]), zu = to_f32<DT>(z[r * n + width + c]);
-            a = g * zu * activate_grad(kActSilu, zg);
-            const float b = g * zg * sigmoid_f(zg);
-            s1 += b;
-            if (dz) dz[r * ldz + width + c] = from_f32<DT>(b);
-        } else if (act != kActNone) {
-            a = g * activate_grad(act, to_f32<DT>(z[r * n + c]));
+    float s0[VEC], s1[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s0[i] = s1[i] = 0.0f;
+    auto read = [&](const uint16_t* p, float* v) {
+        if constexpr (VEC == 4) {
+            const u32v2 w = *(const u32v2*)p;
+            v[0] = to_f32<DT>((uint16_t)w.x), v[1] = to_f32<DT>((uint16_t)(w.x >> 16));
+            v[2] = to_f32<DT>((uint16_t)w.y), v[3] = to_f32<DT>((uint16_t)(w.y >> 16));
+        } else {
+            v[0] = to_f32<DT>(*p);
         }
-        s0 += a;
-        if (dz) dz[r * ldz + c] = from_f32<DT>(a);
+    };
+    auto write = [&](uint16_t* p, const float* v) {
+        if constexpr (VEC == 4) *(u32v2*)p = u32v2{pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3])};
+        else *p = from_f32<DT>(v[0]);
+    };
+    if (c < width) {
+#pragma unroll 2
+        for (int64_t r = r0 + wave; r < r1; r += 4) {
+            float g[VEC], a[VEC];
+            read(dy + r * ldd + c, g);
+            if (act == kActSwiglu) {
+                float zg[VEC], zu[VEC], b[VEC];
+                read(z + r * n + c, zg);
+                read(z + r * n + width + c, zu);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    a[i] = g[i] * zu[i] * activate_grad(kActSilu, zg[i]);
+                    b[i] = g[i] * zg[i] * sigmoid_f(zg[i]);
+                    s1[i] += b[i];
+                }
+                if (dz) write(dz + r * ldz + width + c, b);
+            } else if (act != kActNone) {
+                float v[VEC];
+                read(z + r * n + c, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) a[i] = g[i] * activate_grad(act, v[i]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) a[i] = g[i];
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s0[i] += a[i];
+            if (dz) write(dz + r * ldz + c, a);
+        }
+    } else if (dz) {  // the padding's columns, by the threads behind the last column
+        for (int i = 0; i < VEC; ++i) {
+            const int64_t pad = n + (c - width) + i;
+            if (pad < ldz)
+                for (int64_t r = r0 + wave; r < r1; r += 4) dz[r * ldz + pad] = 0;
+        }
     }
-    if (sums) {
-        sums[blockIdx.y * n + c] = s0;
-        if (act == kActSwiglu) sums[blockIdx.y * n + width + c] = s1;
+    if (!sums) return;
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) part[wave - 1][i][lane] = s0[i], part[wave - 1][VEC + i][lane] = s1[i];
+    }
+    __syncthreads();
+    if (wave == 0 && c < width) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            for (int w = 0; w < 3; ++w) s0[i] += part[w][i][lane], s1[i] += part[w][VEC + i][lane];
+            sums[blockIdx.y * n + c + i] = s0[i];
+            if (act == kActSwiglu) sums[blockIdx.y * n + width + c + i] = s1[i];
+        }
     }
 }
 
+// a wave of 64 columns; the chunks in four parts, one per wave, joined in order
 template <int DT>
 __global__ __launch_bounds__(256) void k_sum_chunks(const float* __restrict__ sums, int64_t chunks, int64_t n, uint16_t* __restrict__ out) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
+    __shared__ float part[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane, per = (chunks + 3) / 4;
+    const int64_t i1 = (wave + 1) * per < chunks ? (wave + 1) * per : chunks;
     float s = 0.0f;
-    for (int64_t i = 0; i < chunks; ++i) s += sums[i * n + c];
-    out[c] = from_f32<DT>(s);
+    if (c < n) {
+#pragma unroll 8
+        for (int64_t i = wave * per; i < i1; ++i) s += sums[i * n + c];
+    }
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < n) out[c] = from_f32<DT>(part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- host
@@ -197,27 +287,23 @@ template <int DT>
 int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
     const int64_t kp = round64(w.k), total_rows = w.experts * w.n, groups = w.k / w.gs;
     const bool fast = aligned_groups(w);
-    const int64_t blocks = fast ? (total_rows + kDequantRows - 1) / kDequantRows : (total_rows * kp + 255) / 256;
+    int log_lanes = 3;
+    while (log_lanes < 8 && (8ll << log_lanes) < kp) ++log_lanes;
+    const int64_t per_block = (256 >> log_lanes) * kDequantRows;
+    const int64_t blocks = fast ? (total_rows + per_block - 1) / per_block : (total_rows * kp + 255) / 256;
     if (blocks > 0x7fffffff) {
         set_error("linear: weight too large");
         return NNCF_AMD_ERR_UNSUPPORTED;
     }
-    const uint32_t vecs = (uint32_t)(kp / 8), per_group = (uint32_t)(w.gs / 8 ? w.gs / 8 : 1);
-    // ceil(2^32 / d); d == 1 would need 2^32 itself: one row of one vector, or groups of 8, take the other kernel
-    const bool magic = fast && vecs > 1 && per_group > 1;
-    const int64_t blocks_any = (total_rows * kp + 255) / 256;
-    if (!magic && blocks_any > 0x7fffffff) {
-        set_error("linear: weight too large");
-        return NNCF_AMD_ERR_UNSUPPORTED;
-    }
-    const uint32_t mr = magic ? (uint32_t)((((uint64_t)1 << 32) + vecs - 1) / vecs) : 0;
-    const uint32_t mg = magic ? (uint32_t)((((uint64_t)1 << 32) + per_group - 1) / per_group) : 0;
+    // ceil(2^32 / (vectors of a group)): exact below 2^14 vectors; 0 for groups of one vector
+    const uint32_t per_group = (uint32_t)(w.gs / 8);
+    const uint32_t magic = fast && per_group > 1 ? (uint32_t)((((uint64_t)1 << 32) + per_group - 1) / per_group) : 0;
 #define GO(M)                                                                                                                  \
-    if (magic)                                                                                                                 \
+    if (fast)                                                                                                                  \
         hipLaunchKernelGGL((k_dequant_rows<M, DT>), dim3((unsigned)blocks), dim3(256), 0, s, w.codes, w.scale, w.zp, out, total_rows, \
-                           w.n, (uint32_t)w.k, (uint32_t)kp, (uint32_t)groups, mr, mg, rows);                                 \
+                           w.n, (uint32_t)w.k, (uint32_t)kp, (uint32_t)groups, magic, log_lanes, rows);                       \
     else                                                                                                                       \
-        hipLaunchKernelGGL((k_dequant_rows_any<M, DT>), dim3((unsigned)blocks_any), dim3(256), 0, s, w.codes, w.scale, w.zp, out, \
+        hipLaunchKernelGGL((k_dequant_rows_any<M, DT>), dim3((unsigned)blocks), dim3(256), 0, s, w.codes, w.scale, w.zp, out,  \
                            total_rows * kp, w.n, w.k, kp, w.gs, rows);
 #define BY_MODE                                                          \
     switch (w.mode) {                                                    \
@@ -235,7 +321,7 @@ int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t
 
 template <int DT>
 int dequant_transposed(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
-    const int64_t np = round64(w.n), tn = (w.n + 63) / 64, tk = (w.k + 63) / 64;
+    const int64_t np = round64(w.n), tn = (w.n + 63) / 64, tk = (w.k + 64 * kTurns - 1) / (64 * kTurns);
     if (tn > 0x7fffffff || tk > 65535 || w.experts > 65535) {
         set_error("linear: weight too large");
         return NNCF_AMD_ERR_UNSUPPORTED;
@@ -537,7 +623,9 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
     }
     const int64_t width = activation == kActSwiglu ? n / 2 : n;
     const int64_t chunks = (m + kChunkRows - 1) / kChunkRows;
-    const int64_t blocks = (width + (dz ? ldz - n : 0) + 255) / 256;
+    // four columns a thread where every row of every operand allows 8-byte accesses
+    const bool wide = width % 4 == 0 && n % 4 == 0 && ldd % 4 == 0 && (!dz || ldz % 4 == 0) && (((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz) & 7) == 0;
+    const int64_t per = wide ? 256 : 64, blocks = (width + (dz ? ldz - n : 0) + per - 1) / per;
     if (m > 0 && (!dy || ldd < width || (activation != kActNone && !z) || (dz && ldz < n))) {
         set_error("activation_grad: null or overlapping rows (ldd=%lld ldz=%lld)", (long long)ldd, (long long)ldz);
         return NNCF_AMD_ERR_BAD_ARG;
@@ -554,17 +642,22 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
     float* sums = dbias ? (float*)workspace : nullptr;
     if (m > 0 && (dz || dbias)) {
         const dim3 grid((unsigned)blocks, (unsigned)chunks);
-        if (dtype == NNCF_AMD_BF16)
-            hipLaunchKernelGGL((k_activation_grad<NNCF_AMD_BF16>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, (const uint16_t*)z, m, n,
-                               activation, (uint16_t*)dz, ldz, sums);
-        else
-            hipLaunchKernelGGL((k_activation_grad<NNCF_AMD_F16>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, (const uint16_t*)z, m, n,
-                               activation, (uint16_t*)dz, ldz, sums);
+#define GO(DT, VEC)                                                                                                              \
+    hipLaunchKernelGGL((k_activation_grad<DT, VEC>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, (const uint16_t*)z, m, n, \
+                       activation, (uint16_t*)dz, ldz, sums)
+        if (dtype == NNCF_AMD_BF16) {
+            if (wide) GO(NNCF_AMD_BF16, 4);
+            else GO(NNCF_AMD_BF16, 1);
+        } else {
+            if (wide) GO(NNCF_AMD_F16, 4);
+            else GO(NNCF_AMD_F16, 1);
+        }
+#undef GO
         const int st = launch_status("activation_grad");
         if (st != NNCF_AMD_OK) return st;
     }
     if (dbias) {
-        const dim3 grid((unsigned)((n + 255) / 256));
+        const dim3 grid((unsigned)((n + 63) / 64));
         if (dtype == NNCF_AMD_BF16)
             hipLaunchKernelGGL((k_sum_chunks<NNCF_AMD_BF16>), grid, dim3(256), 0, s, sums, chunks, n, (uint16_t*)dbias);
         else
