@@ -5,17 +5,22 @@
 // A block owns a tile of 32 * WI * FA rows of W by 32 * WJ * FB rows of x, WI x WJ waves, each FA x FB accumulators of
 // v_mfma_f32_32x32x16 (W is the A operand: a lane ends with four consecutive columns of one row of y).
 // Both operands go global -> LDS by buffer DMA in stages of 64 k: 128 bytes a row, whole lines (stages of 32 k ask for half
-// lines and fetch each of them twice: 1.0 PFLOP/s where this form reaches the figure at dense_typed).  Two stages: while one is
-// read the other one lands; a barrier in the last quarter of a stage frees it.  A row's 16-byte chunk c sits at chunk position
-// c ^ (row & 7): eight consecutive lanes of a fragment read eight rows and then touch all banks.  The DMA writes LDS linearly,
-// so the permutation is applied to its source.
+// lines and fetch each of them twice).  LDS has five slots for stages of one operand: while a stage is read, the next one and
+// W's of the one after land; a barrier in the last quarter of a stage frees it (two slots per operand: 645 us against 600 for
+// 2000 gathered rows over eight experts of 4096 x 14336).  A row's 16-byte chunk c sits at chunk position c ^ (row / 2 & 7): 16
+// consecutive lanes of a fragment read 16 rows and touch all 64 banks.  The DMA writes LDS linearly, so the permutation is
+// applied to its source.
+//
+// A stage of 64 k takes 2250 clocks of the 2048 that its matrix instructions need; what bounds it is power: the clock goes down
+// to 1.6-1.7 GHz while it runs (2.1 with the DMA taken out).  The epilogue takes 5 us a tile, 8 columns per lane (30 us when each
+// lane took 4 and chose the activation per element).
 #include <type_traits>
 
 #include "wc_linear.h"
 
 namespace wc {
 
-constexpr int kStages = 2;
+constexpr int kSlots = 5;       // of LDS: a stage of one operand each
 constexpr int kRowBytes = 128;  // 64 k of 16 bits
 
 // written out: through the builtin the compiler sees an LDS store of unknown address and waits for it at every LDS read
@@ -33,8 +38,25 @@ __device__ __forceinline__ i32x4 uniform(i32x4 v) {
     return i32x4{__builtin_amdgcn_readfirstlane(v.x), __builtin_amdgcn_readfirstlane(v.y), __builtin_amdgcn_readfirstlane(v.z),
                  __builtin_amdgcn_readfirstlane(v.w)};
 }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
 
-// Tiles of rows: expert e has ceil(rows / PB) of them, in order.  Tile `t` -> its expert and first row; false behind the last.
+// Tiles of rows: expert e has ceil(rows / PB) of them, in order.  How many there are, `most` at most.
+template <int PB>
+__device__ __forceinline__ uint32_t count_tiles(const RowMap& r, uint32_t most) {
+    const int lane = threadIdx.x & 63;
+    int64_t sum = 0;
+    for (int e = lane; e < r.experts; e += 64) {
+        int64_t lo, hi;
+        expert_range(r, e, lo, hi);
+        sum += (hi - lo + PB - 1) / PB;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+    return (uint32_t)uniform(sum < (int64_t)most ? sum : (int64_t)most);
+}
+// Tile `t` -> its expert and first row; false behind the last.
 template <int PB>
 __device__ __forceinline__ bool find_tile(const RowMap& r, int64_t t, int& expert, int64_t& first, int64_t& last) {
     if (!r.offsets) {
@@ -68,18 +90,105 @@ __device__ __forceinline__ bool find_tile(const RowMap& r, int64_t t, int& exper
     return false;
 }
 
+// 32 rows of sums in LDS -> y, where all the columns are inside and their addresses allow vectors: LANES lanes per row, 8
+// columns each, so that a lane keeps its columns' bias, and four of its rows of the residual are requested before the first is needed.
+template <int DT, int ACT, int LANES, int PITCH>
+__device__ __forceinline__ void finish_rows(const Epilogue& e, const float* tile, int64_t row0, int64_t last, int64_t col0, uint32_t lane) {
+    typedef uint32_t halves8 __attribute__((ext_vector_type(4), aligned(8)));
+    constexpr bool GATED = ACT == kActSwiglu;
+    constexpr int ROWS = 64 / LANES, TURNS = 32 / ROWS, AT_ONCE = TURNS < 4 ? TURNS : 4;
+    const int64_t width = GATED ? e.n / 2 : e.n, col = col0 + lane % LANES * 8;
+    const uint32_t r0 = lane / LANES;
+    float bz[8] = {}, bu[GATED ? 8 : 1] = {};
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            bz[i] = to_f32<DT>(((const uint16_t*)e.bias)[col + i]);
+            if constexpr (GATED) bu[i] = to_f32<DT>(((const uint16_t*)e.bias)[width + col + i]);
+        }
+    }
+    auto pack = [](const float* v) { return halves8{pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3]), pair_of<DT>(v[4], v[5]), pair_of<DT>(v[6], v[7])}; };
+#pragma unroll 1
+    for (int t0 = 0; t0 < TURNS; t0 += AT_ONCE) {
+        halves8 res[AT_ONCE];
+        if (e.residual) {
+#pragma unroll
+            for (int t = 0; t < AT_ONCE; ++t) {
+                const int64_t row = row0 + (t0 + t) * ROWS + r0;
+                res[t] = *(const halves8*)((const uint16_t*)e.residual + (row < last ? row : last - 1) * e.ldr + col);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) {
+            const uint32_t r = (t0 + t) * ROWS + r0;
+            const int64_t row = row0 + r;
+            const float* at = tile + r * PITCH + lane % LANES * 8;
+            float z[8], u[GATED ? 8 : 1], v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                z[i] = at[i] + bz[i];
+                if constexpr (GATED) u[i] = at[LANES * 8 + i] + bu[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (GATED) v[i] = z[i] * sigmoid_f(z[i]) * u[i];
+                else v[i] = activate(ACT, z[i]);
+            }
+            if (row >= last) continue;
+            if (e.y32) {
+                float* y = (float*)e.y + row * e.ldy + col;
+                *(f32x4*)y = f32x4{v[0], v[1], v[2], v[3]}, *(f32x4*)(y + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                continue;
+            }
+            if (e.residual) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[2 * j] += to_f32<DT>((uint16_t)res[t][j]), v[2 * j + 1] += to_f32<DT>((uint16_t)(res[t][j] >> 16));
+            }
+            *(halves8*)((uint16_t*)e.y + row * e.ldy + col) = pack(v);
+            if (e.z) {
+                uint16_t* z_at = (uint16_t*)e.z + row * e.n + col;
+                *(halves8*)z_at = pack(z);
+                if constexpr (GATED) *(halves8*)(z_at + width) = pack(u);
+            }
+        }
+    }
+}
+
 template <int DT, int WI, int WJ, int FA, int FB>
 __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t tiles_m, uint32_t tiles_n) {
     constexpr int NW = WI * WJ, PA = 32 * WI * FA, PB = 32 * WJ * FB;  // waves; tile rows of W and of x
-    constexpr int kStageBytes = (PA + PB) * kRowBytes;
+    static_assert(PA == PB, "the operands' stages take each other's slots");
+    constexpr int kSlotBytes = PA * kRowBytes;
     constexpr int DA = PA / (8 * NW), DB = PB / (8 * NW), NDMA = DA + DB;  // DMA instructions per wave and stage: 8 rows each
     static_assert(PA % (8 * NW) == 0 && PB % (8 * NW) == 0, "every wave brings in whole instructions' rows");
     extern __shared__ __align__(16) char smem[];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wi = wave / WJ, wj = wave % WJ;
 
+    const bool gated = g.ep.act == kActSwiglu;
+    const int64_t width = gated ? g.ep.n / 2 : g.ep.n;
+    if (g.rows.offsets) {  // rows behind the last group are zero: every block of the grid takes its share
+        int64_t lo, hi;
+        expert_range(g.rows, g.rows.experts - 1, lo, hi);
+        const int64_t col = (int64_t)(blockIdx.x % tiles_n) * (gated ? PA / 2 : PA);
+        const int64_t end = col + (gated ? PA / 2 : PA) < width ? col + (gated ? PA / 2 : PA) : width;
+        const uint32_t at = blockIdx.x / tiles_n;
+        if (at < tiles_m)
+            for (int64_t r = hi + at; r < g.rows.rows; r += tiles_m)
+                for (int64_t c = col + threadIdx.x; c < end; c += 64 * NW) {
+                    if (g.ep.y32) ((float*)g.ep.y)[r * g.ep.ldy + c] = 0.0f;
+                    else ((uint16_t*)g.ep.y)[r * g.ep.ldy + c] = 0;
+                    if (g.ep.z) {
+                        ((uint16_t*)g.ep.z)[r * g.ep.n + c] = 0;
+                        if (gated) ((uint16_t*)g.ep.z)[r * g.ep.n + width + c] = 0;
+                    }
+                }
+        tiles_m = count_tiles<PB>(g.rows, tiles_m);
+    }
+
     // Tiles in bands of 8 row tiles, the row tile fastest inside a band; the workgroups of one XCD (they are dealt out in
-    // turn over the 8 of them) take a run of consecutive tiles, so that its L2 holds 8 strips of x and a few of W.
+    // turn over the 8 of them) take a run of consecutive tiles, so that its L2 holds 8 strips of x and a few of W.  Ragged
+    // groups: of the tiles that there are, since the grid has as many as there could be.
     const uint32_t total = tiles_m * tiles_n;
     const uint32_t per = (total + 7) / 8;
     const uint32_t id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -87,28 +196,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
     const uint32_t band = id / (8 * tiles_n), in_band = id - band * 8 * tiles_n;
     const uint32_t wide = tiles_m - 8 * band < 8 ? tiles_m - 8 * band : 8;
     const uint32_t tm = 8 * band + in_band % wide, tn = in_band / wide;
-
-    const bool gated = g.ep.act == kActSwiglu;
-    const int64_t width = gated ? g.ep.n / 2 : g.ep.n;
     const int64_t col0 = (int64_t)tn * (gated ? PA / 2 : PA);
 
-    if (g.rows.offsets) {  // rows behind the last group are zero: every row tile's block takes its share
-        int64_t lo, hi;
-        expert_range(g.rows, g.rows.experts - 1, lo, hi);
-        const int64_t end = col0 + (gated ? PA / 2 : PA) < width ? col0 + (gated ? PA / 2 : PA) : width;
-        for (int64_t r = hi + tm; r < g.rows.rows; r += tiles_m)
-            for (int64_t c = col0 + threadIdx.x; c < end; c += 64 * NW) {
-                if (g.ep.y32) ((float*)g.ep.y)[r * g.ep.ldy + c] = 0.0f;
-                else ((uint16_t*)g.ep.y)[r * g.ep.ldy + c] = 0;
-                if (g.ep.z) {
-                    ((uint16_t*)g.ep.z)[r * g.ep.n + c] = 0;
-                    if (gated) ((uint16_t*)g.ep.z)[r * g.ep.n + width + c] = 0;
-                }
-            }
-    }
     int expert;
     int64_t first, last;
     if (!find_tile<PB>(g.rows, tm, expert, first, last)) return;
+    first = uniform(first), last = uniform(last);
 
     // sources of this lane's DMA chunks: instruction u of the wave fills 8 consecutive tile rows
     const char* wbase = (const char*)g.w + (int64_t)expert * g.ep.n * g.k * 2;
@@ -122,7 +215,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
     for (int u = 0; u < NDMA; ++u) {
         const bool is_w = u < DA;
         const uint32_t at8 = ((is_w ? u : u - DA) * NW + wave) * 8, row = at8 + (lane >> 3);  // row in the operand's tile
-        const uint32_t chunk = (lane & 7) ^ (row & 7);
+        const uint32_t chunk = (lane & 7) ^ (row >> 1 & 7);
         int64_t at;
         if (is_w) {
             int64_t c;
@@ -142,25 +235,30 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
             at = (source_row(g.rows, r) - xorg) * g.ldx * 2;
         }
         voff[u] = (uint32_t)at + chunk * 16;
-        dst[u] = ((is_w ? 0 : PA) + at8) * kRowBytes;
+        dst[u] = at8 * kRowBytes;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
     const int nst = (int)(g.k / 64);
-    uint32_t so = 0, lds_st = 0;
-    auto issue_prepare = [&](int st) {
-        so = (uint32_t)st * kRowBytes;
-        lds_st = lds0 + (uint32_t)(st % kStages) * kStageBytes;
+    // Slots of a stage, going round: W's 2 st, x's 2 st + 1 (modulo 5).  So W's stage may come in one stage earlier than x's.
+    uint32_t so_w = 0, so_x = 0, slot_w = 0, slot_x = 0;
+    auto issue_prepare = [&](int st_x, int st_w) {  // x's stage and W's stage that are brought in next
+        so_x = (uint32_t)st_x * kRowBytes, so_w = (uint32_t)st_w * kRowBytes;
+        slot_x = lds0 + (uint32_t)(2 * st_x + 1) % kSlots * kSlotBytes, slot_w = lds0 + (uint32_t)(2 * st_w) % kSlots * kSlotBytes;
     };
-    auto issue_one = [&](int u) { dma16(u < DA ? rw : rx, voff[u], so, lds_st + dst[u]); };
+    // u < DB: x's instructions, then W's
+    auto issue_one = [&](int u) {
+        if (u < DB) dma16(rx, voff[DA + u], so_x, slot_x + dst[DA + u]);
+        else dma16(rw, voff[u - DB], so_w, slot_w + dst[u - DB]);
+    };
 
     typedef int op_t __attribute__((ext_vector_type(4)));
     const uint32_t r32 = lane & 31, kh = lane >> 5;
     uint32_t offa[4], offb[4];  // per quarter of the stage; the fragments follow 32 rows apart (32 rows keep the permutation)
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
-        const uint32_t at = r32 * kRowBytes + (((2 * ks + kh) ^ (r32 & 7)) * 16);
+        const uint32_t at = r32 * kRowBytes + (((2 * ks + kh) ^ (r32 >> 1 & 7)) * 16);
         offa[ks] = wi * 32 * FA * kRowBytes + at;
-        offb[ks] = (PA + wj * 32 * FB) * kRowBytes + at;
+        offb[ks] = wj * 32 * FB * kRowBytes + at;
     }
     auto read_op = [&](const char* img, uint32_t off) { return *(const op_t*)(img + off); };
     f32x16 acc[FA][FB];
@@ -180,12 +278,14 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
     constexpr int kSync = 1;                // MFMAs of a stage's last quarter in front of the barrier
     constexpr int kFirst = NM - kSync - 1;  // DMA instructions of a stage that go into the last quarter before it; the rest follows
     op_t a0[FA], b0[FB], a1[FA], b1[FB];
-    // 16 k: the MFMAs on (ca, cb) and between them the LDS reads of the next 16 k from `img`, quarter KS of its stage.  KS == 0
-    // means the last quarter of the stage before: first the barrier (the other stage has landed, and nobody reads this one any
-    // more), then the DMA of the stage after next into its place.  DMA: instructions of it that are issued here, from D0 on.
-    auto kstep = [&](const op_t* ca, const op_t* cb, op_t* na, op_t* nb, const char* img, auto ks, auto reads, auto d0, auto d1) {
+    // 16 k: the MFMAs on (ca, cb) and between them the LDS reads of the next 16 k, quarter KS of the stage at (imga, imgb).
+    // KS == 0 means the last quarter of the stage before: first the barrier (the stage that follows has landed, at most `OUT`
+    // instructions of later ones are on their way, and nobody reads this stage any more), then the DMA into its slots.
+    // D0 ... D1: instructions of it that are issued here.
+    auto kstep = [&](const op_t* ca, const op_t* cb, op_t* na, op_t* nb, const char* imga, const char* imgb, auto ks, auto reads, auto out,
+                     auto d0, auto d1) {
         constexpr bool READS = decltype(reads)::value;
-        constexpr int KS = decltype(ks)::value, D0 = decltype(d0)::value, D1 = decltype(d1)::value;
+        constexpr int KS = decltype(ks)::value, OUT = decltype(out)::value, D0 = decltype(d0)::value, D1 = decltype(d1)::value;
         constexpr int R0 = KS == 0 && READS ? kSync + 1 : 0;  // MFMA behind which the reads begin
         constexpr int kPerSlot = (NR + NM - R0 - 1) / (NM - R0);
         constexpr int kDmaPerSlot = D1 > D0 ? (D1 - D0 + NM - R0 - 1) / (NM - R0) : 0;
@@ -194,7 +294,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
             mfma(acc[i / FB][i % FB], ca[i / FB], cb[i % FB]);
             if constexpr (KS == 0 && READS) {
                 if (i == kSync) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(OUT) : "memory");
                     __builtin_amdgcn_s_barrier();
                 }
             }
@@ -203,8 +303,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
                 for (int j = 0; j < kPerSlot; ++j) {
                     const int r = (i - R0) * kPerSlot + j;
                     if (i < R0 || r >= NR) continue;
-                    if (r < FA) na[r] = read_op(img, offa[KS] + r * 32 * kRowBytes);
-                    else nb[r - FA] = read_op(img, offb[KS] + (r - FA) * 32 * kRowBytes);
+                    if (r < FA) na[r] = read_op(imga, offa[KS] + r * 32 * kRowBytes);
+                    else nb[r - FA] = read_op(imgb, offb[KS] + (r - FA) * 32 * kRowBytes);
                 }
             }
             if constexpr (D1 > D0) {
@@ -219,43 +319,48 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
     using T = std::true_type;
     using F = std::false_type;
 #define N_(v) std::integral_constant<int, (v)>{}
-    constexpr int kHead = NDMA < 2 * kFirst ? (NDMA + 1) / 2 : kFirst;  // of a stage's DMA in the quarter behind the barrier
-    issue_prepare(0);
+    auto slot_at = [&](int i) { return smem + (uint32_t)i % kSlots * kSlotBytes; };
+    // A stage's DMA (x's of two stages on, W's of three) begins behind its barrier: kHead instructions of it in the last
+    // quarter, the rest in the first of the next.  In front of the loop (there are at least three stages): both operands'
+    // first, W's second, and the head of what the stage before the first would have begun.
+    constexpr int kHead = (NDMA + 3) / 4, kTwo = (NDMA + 1) / 2, kThree = kTwo + kHead < NDMA ? kTwo + kHead : NDMA;
+    issue_prepare(0, 0);
 #pragma unroll
     for (int u = 0; u < NDMA; ++u) issue_one(u);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    issue_prepare(0, 1);
+#pragma unroll
+    for (int u = DB; u < NDMA; ++u) issue_one(u);
+    issue_prepare(1, 2);
+#pragma unroll
+    for (int u = 0; u < kHead; ++u) issue_one(u);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(DA + kHead) : "memory");
     __builtin_amdgcn_s_barrier();
-    if (nst > 1) {
-        issue_prepare(1);
 #pragma unroll
-        for (int u = 0; u < kHead; ++u) issue_one(u);
-    }
+    for (int m = 0; m < FA; ++m) a0[m] = read_op(slot_at(0), offa[0] + m * 32 * kRowBytes);
 #pragma unroll
-    for (int m = 0; m < FA; ++m) a0[m] = read_op(smem, offa[0] + m * 32 * kRowBytes);
-#pragma unroll
-    for (int m = 0; m < FB; ++m) b0[m] = read_op(smem, offb[0] + m * 32 * kRowBytes);
+    for (int m = 0; m < FB; ++m) b0[m] = read_op(slot_at(1), offb[0] + m * 32 * kRowBytes);
     int st = 0;
-    for (; st + 2 < nst; ++st) {
-        const char* img = smem + (st & 1) * kStageBytes;
-        kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(kHead), N_(NDMA));
-        kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
-        kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
-        issue_prepare(st + 2);
-        kstep(a1, b1, a0, b0, smem + ((st + 1) & 1) * kStageBytes, N_(0), T{}, N_(0), N_(kHead));
+    auto quarters = [&](auto more) {
+        constexpr int M = decltype(more)::value;
+        const char *ia = slot_at(2 * st), *ib = slot_at(2 * st + 1);
+        kstep(a0, b0, a1, b1, ia, ib, N_(1), T{}, N_(0), N_(M * kHead), N_(M * kTwo));
+        kstep(a1, b1, a0, b0, ia, ib, N_(2), T{}, N_(0), N_(M * kTwo), N_(M * kThree));
+        kstep(a0, b0, a1, b1, ia, ib, N_(3), T{}, N_(0), N_(M * kThree), N_(M * NDMA));
+    };
+    for (; st + 3 < nst; ++st) {
+        quarters(N_(1));
+        issue_prepare(st + 2, st + 3);
+        kstep(a1, b1, a0, b0, slot_at(2 * st + 2), slot_at(2 * st + 3), N_(0), T{}, N_(DA), N_(0), N_(kHead));
     }
-    if (st + 1 < nst) {
-        const char* img = smem + (st & 1) * kStageBytes;
-        kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(kHead), N_(NDMA));
-        kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
-        kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
-        kstep(a1, b1, a0, b0, smem + ((st + 1) & 1) * kStageBytes, N_(0), T{}, N_(0), N_(0));
-        ++st;
-    }
-    const char* img = smem + (st & 1) * kStageBytes;
-    kstep(a0, b0, a1, b1, img, N_(1), T{}, N_(0), N_(0));
-    kstep(a1, b1, a0, b0, img, N_(2), T{}, N_(0), N_(0));
-    kstep(a0, b0, a1, b1, img, N_(3), T{}, N_(0), N_(0));
-    kstep(a1, b1, a0, b0, img, N_(0), F{}, N_(0), N_(0));
+    quarters(N_(1));
+    issue_prepare(st + 2, st + 2);
+    kstep(a1, b1, a0, b0, slot_at(2 * st + 2), slot_at(2 * st + 3), N_(0), T{}, N_(DA), N_(0), N_(DB));  // x's only
+    ++st;
+    quarters(N_(0));
+    kstep(a1, b1, a0, b0, slot_at(2 * st + 2), slot_at(2 * st + 3), N_(0), T{}, N_(0), N_(0), N_(0));
+    ++st;
+    quarters(N_(0));
+    kstep(a1, b1, a0, b0, smem, smem, N_(0), F{}, N_(0), N_(0), N_(0));
 #undef N_
     asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // the last MFMAs leave the pipe before the read-out
 
@@ -266,16 +371,36 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
     __syncthreads();
     const uint32_t cols = gated ? 16 * FA : 32 * FA;  // of y
     const int64_t col_w = col0 + wi * cols;
-#pragma unroll
+    const bool whole = g.ep.vec && col_w + cols <= width;
+#pragma unroll 1
     for (int b = 0; b < FB; ++b) {
 #pragma unroll
-        for (int a = 0; a < FA; ++a)
+        for (int bb = 0; bb < FB; ++bb) {
+            if (bb != b) continue;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *(f32x4*)(tile + r32 * kPitch + a * 32 + 8 * q + 4 * kh) =
-                    f32x4{acc[a][b][4 * q], acc[a][b][4 * q + 1], acc[a][b][4 * q + 2], acc[a][b][4 * q + 3]};
-        const int64_t row0 = first + wj * 32 * FB + b * 32;
-        for (uint32_t i = lane * 4; i < 32 * cols; i += 256) {  // (the wave's own floats: no barrier)
+            for (int a = 0; a < FA; ++a)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(f32x4*)(tile + r32 * kPitch + a * 32 + 8 * q + 4 * kh) =
+                        f32x4{acc[a][bb][4 * q], acc[a][bb][4 * q + 1], acc[a][bb][4 * q + 2], acc[a][bb][4 * q + 3]};
+        }
+        const int64_t row0 = first + wj * 32 * FB + b * 32;  // (the wave's own floats: no barrier)
+        if (row0 >= last) break;
+        if (whole) {
+#define FINISH(ACT, LANES) \
+    case ACT: finish_rows<DT, ACT, LANES, kPitch>(g.ep, tile, row0, last, col_w, lane); break;
+            switch (g.ep.act) {
+                FINISH(kActNone, 4 * FA)
+                FINISH(kActRelu, 4 * FA)
+                FINISH(kActGelu, 4 * FA)
+                FINISH(kActGeluTanh, 4 * FA)
+                FINISH(kActSilu, 4 * FA)
+                FINISH(kActSwiglu, 2 * FA)
+            }
+#undef FINISH
+            continue;
+        }
+        for (uint32_t i = lane * 4; i < 32 * cols; i += 256) {
             const uint32_t r = i / cols, c = i % cols;
             if (row0 + r >= last) break;
             const f32x4 s = *(const f32x4*)(tile + r * kPitch + c);
@@ -289,7 +414,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
 template <int DT, int WI, int WJ, int FA, int FB>
 int dense_tiles(const DenseArgs& a, hipStream_t s) {
     static OncePerDevice once;
-    constexpr int PA = 32 * WI * FA, PB = 32 * WJ * FB, kStageLds = kStages * (PA + PB) * kRowBytes;
+    constexpr int PA = 32 * WI * FA, PB = 32 * WJ * FB, kStageLds = kSlots * PA * kRowBytes;
     constexpr int kTileLds = WI * WJ * 32 * (32 * FA + 4) * 4;  // the epilogue's floats take the stages' place
     constexpr int kLds = kStageLds > kTileLds ? kStageLds : kTileLds;
     const int first = once.first_on_device();
@@ -322,9 +447,10 @@ bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gate
     return (gated ? n : 512) * k * 2 < kMost && (gathered ? sources : 512) * ldx * 2 < kMost;
 }
 
-// 256 x 256 tiles by eight waves (1.28 PFLOP/s on 4096 x 28672 x 8192, one block per compute unit) or 128 x 128 by four (0.98,
-// two blocks): whichever needs less time in rounds of blocks, a round of the small ones costing two thirds of one of the
-// large ones (2047 x 4096 x 4096: 128 large tiles 110 us, 512 small ones 90; 4096 x 4096 x 4096: 141 against 158).
+// 256 x 256 tiles by eight waves (1.38 PFLOP/s on 4096 x 28672 x 8192, one block per compute unit) or 128 x 128 by four (1.10,
+// two blocks): whichever needs less time in rounds of blocks, a round of the small ones costing 0.6 of one of the large ones
+// (4096 x 4096 x 4096: one round of large tiles 108 us, two of small ones 125; 2047 rows: 68 us in 512 small ones, 83 in 128
+// large ones, half a round).
 template <int DT>
 int dense_typed(const DenseArgs& a, hipStream_t s) {
     const int64_t width = a.ep.n, groups = a.rows.offsets ? a.rows.experts : 1;
@@ -332,7 +458,7 @@ int dense_typed(const DenseArgs& a, hipStream_t s) {
         const int64_t rows = (a.rows.rows + tile - 1) / tile + (groups - 1) / 2;  // ragged groups: half a tile each on average
         return ((width + tile - 1) / tile * rows + at_once - 1) / at_once;
     };
-    if (3 * rounds(256, 256) <= 2 * rounds(128, 512)) return dense_tiles<DT, 2, 4, 4, 2>(a, s);
+    if (5 * rounds(256, 256) <= 3 * rounds(128, 512)) return dense_tiles<DT, 2, 4, 4, 2>(a, s);
     return dense_tiles<DT, 2, 2, 2, 2>(a, s);
 }
 

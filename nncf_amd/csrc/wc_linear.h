@@ -301,7 +301,7 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
     }
 }
 
-// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 64 and 16-byte rows, w [experts * n, k]
+// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 64, 192 at least, and 16-byte rows, w [experts * n, k]
 struct DenseArgs {
     const void* x;
     const void* w;

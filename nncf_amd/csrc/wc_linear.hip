@@ -8,10 +8,11 @@
 
 namespace wc {
 
-constexpr int64_t round64(int64_t v) { return (v + 63) / 64 * 64; }
+// k as the dense product takes it: stages of 64, three at least
+constexpr int64_t padded(int64_t v) { return v <= 192 ? 192 : (v + 63) / 64 * 64; }
 
 // ---------------------------------------------------------------------------------- weight -> dense rows of the workspace
-// [experts * n, kp], kp = k rounded up to 64, the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  `lanes` (a
+// [experts * n, kp], kp = k rounded up to 64 (192 at least), the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  `lanes` (a
 // power of two) threads follow a row, 8 weights each; a thread takes the same place of kDequantRows rows, whose reads are
 // requested together and whose addresses are a scalar apart.  An expert without rows is left out.
 constexpr int kDequantRows = 4;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256) void k_dequant_rows_any(const uint8_t* __restr
 }
 
 // ------------------------------------------------------------------------- weight -> its transpose, for the gradient of x
-// [experts, k, np], np = n rounded up to 64, the tail zero: tiles of 64 x 64 turned round in LDS as pairs of neighbouring n
+// [experts, k, np], np = n rounded up to 64 (192 at least), the tail zero: tiles of 64 x 64 turned round in LDS as pairs of neighbouring n
 // (rows padded by 4 bytes so that the columns that are written fall on different banks).
 constexpr int kTurns = 4;
 template <int MODE, int DT, bool ALIGNED>
@@ -285,7 +286,7 @@ bool aligned_groups(const Weight& w) {  // 8 consecutive weights of a row: one g
 
 template <int DT>
 int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
-    const int64_t kp = round64(w.k), total_rows = w.experts * w.n, groups = w.k / w.gs;
+    const int64_t kp = padded(w.k), total_rows = w.experts * w.n, groups = w.k / w.gs;
     const bool fast = aligned_groups(w);
     int log_lanes = 3;
     while (log_lanes < 8 && (8ll << log_lanes) < kp) ++log_lanes;
@@ -321,7 +322,7 @@ int dequant_rows(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t
 
 template <int DT>
 int dequant_transposed(const Weight& w, const RowMap& rows, uint16_t* out, hipStream_t s) {
-    const int64_t np = round64(w.n), tn = (w.n + 63) / 64, tk = (w.k + 64 * kTurns - 1) / (64 * kTurns);
+    const int64_t np = padded(w.n), tn = np / 64, tk = (w.k + 64 * kTurns - 1) / (64 * kTurns);
     if (tn > 0x7fffffff || tk > 65535 || w.experts > 65535) {
         set_error("linear: weight too large");
         return NNCF_AMD_ERR_UNSUPPORTED;
@@ -386,23 +387,23 @@ struct Need {
     FewShape shape;
     size_t total() const { return weight + pack; }
 };
-// The time of the other way, in the units of FewShape: the weight decompressed (2.6 bytes an element at 5 TB/s) and multiplied
-// by 128 x 128 or 256 x 256 tiles (1.1 and 1.7 us for 64 k of a round of blocks, the former 0.65 where half the blocks fill it).
+// The time of the other way, in the units of FewShape: the weight decompressed (2.6 bytes an element at 6 TB/s) and multiplied
+// by 128 x 128 or 256 x 256 tiles (1 and 1.6 us for 64 k of a round of blocks, the former 0.6 where half the blocks fill it).
 // 28672 x 8192: codes 144 us against 280 for 128 rows, 270 against 300 for 256, 520 against 365 for 512.
 int64_t dense_cost(const Weight& w, int64_t rows, bool grouped) {
     auto blocks = [&](int64_t tile) { return ((w.n + tile - 1) / tile) * ((rows + tile - 1) / tile + (grouped ? (w.experts - 1) / 2 : 0)); };
     const int64_t small = blocks(128), large = blocks(256), steps = (w.k + 63) / 64;
-    const double t128 = small <= 256 ? 0.65 : 1.1 * (double)((small + 511) / 512), t256 = 1.7 * (double)((large + 255) / 256);
-    const double us = (double)w.experts * (double)w.n * (double)w.k * 2.6 / 5.0e6 + (double)steps * (t128 < t256 ? t128 : t256) + 8.0;
+    const double t128 = small <= 256 ? 0.6 : (double)((small + 511) / 512), t256 = 1.6 * (double)((large + 255) / 256);
+    const double us = (double)w.experts * (double)w.n * (double)w.k * 2.6 / 6.0e6 + (double)steps * (t128 < t256 ? t128 : t256) + 8.0;
     return (int64_t)(us / 0.12);
 }
 bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gathered) {
-    return k % 64 || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
+    return k != padded(k) || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
 }
 Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows, bool gated, bool grouped) {
-    Need d{(size_t)(w.experts * w.n * round64(w.k)) * 2, 0, false, {}};
+    Need d{(size_t)(w.experts * w.n * padded(w.k)) * 2, 0, false, {}};
     const bool copy = ldx % 8 || ((uintptr_t)x & 15);
-    d.few = rows <= 1024 * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? round64(w.k) : ldx);
+    d.few = rows <= 1024 * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? padded(w.k) : ldx);
     if (d.few) {
         d.shape = few_plan(w.mode, w.n, w.k, w.k / w.gs, gated, rows, w.experts, grouped);
         d.few = d.shape.cost < dense_cost(w, rows, grouped);
@@ -410,12 +411,12 @@ Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, 
     if (d.few) {
         d.weight = d.shape.kz > 1 ? (size_t)(d.shape.kz * rows * w.n + 3) / 4 * 16 : 0;
     }
-    if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * round64(w.k)) * 2;
+    if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * padded(w.k)) * 2;
     return d;
 }
 Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
-    Need d{(size_t)(w.experts * w.k * round64(w.n)) * 2, 0, false, {}};
-    if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * round64(w.n)) * 2;
+    Need d{(size_t)(w.experts * w.k * padded(w.n)) * 2, 0, false, {}};
+    if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * padded(w.n)) * 2;
     return d;
 }
 
@@ -427,7 +428,7 @@ int vec_of(const Epilogue& e) {
 }
 
 int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* pack, hipStream_t s) {
-    const int64_t kp = round64(k);
+    const int64_t kp = padded(k);
     if (rows.rows > 0x7fffffff) {
         set_error("linear: too many rows");
         return NNCF_AMD_ERR_UNSUPPORTED;
@@ -438,7 +439,7 @@ int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* p
 }
 
 int run_dense(int dtype, const void* x, int64_t ldx, int64_t k, const void* w, RowMap rows, Epilogue ep, uint16_t* pack, hipStream_t s) {
-    const int64_t kp = round64(k);
+    const int64_t kp = padded(k);
     if (must_pack(x, ldx, k, rows.sources, rows.slots != nullptr)) {
         const int st = pack_rows(x, ldx, k, rows, pack, s);
         if (st != NNCF_AMD_OK) return st;
