@@ -17,11 +17,11 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
          "-Wall", "-Wno-unused-function", "-Wno-inline-asm"]
 # per-file additions.  wc_cholinv.hip: the SLP vectoriser pairs the rank-16 updates of the panel kernel into v_pk_fma_f32
 # and pays for it with ~2300 register moves and 110 more registers (15 000 -> 13 300 instructions per wave without it)
-# wc_linear*.hip, wc_gemm_nt.hip, wc_experts.hip: no packed fp32 instructions, some of whose forms are not dependable on this
+# wc_linear*.hip, wc_gemm_*.hip, wc_experts.hip: no packed fp32 instructions, some of whose forms are not dependable on this
 # hardware (the host pass does not know the feature and says so)
 _NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FILE_FLAGS = {"wc_cholinv.hip": ["-fno-slp-vectorize"], "wc_linear.hip": _NO_PACKED_FP32, "wc_gemm_nt.hip": _NO_PACKED_FP32,
-              "wc_linear_few.hip": _NO_PACKED_FP32, "wc_experts.hip": _NO_PACKED_FP32}
+              "wc_gemm_codes.hip": _NO_PACKED_FP32, "wc_linear_few.hip": _NO_PACKED_FP32, "wc_experts.hip": _NO_PACKED_FP32}
 
 
 def sources():

@@ -351,5 +351,30 @@ bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t source
 // the quickest shape for `rows` rows of x over `experts` weights (grouped: with row offsets)
 FewShape few_plan(int mode, int64_t n, int64_t k, int64_t groups, bool gated, int64_t rows, int64_t experts, bool grouped);
 int few_launch(int dtype, int mode, const FewArgs& a, const FewShape& sh, hipStream_t s);
+// y from the sums [kz][rows][n] that blocks sharing k left, in the order of their parts
+int join_sums(int dtype, const float* sums, int kz, const RowMap& rows, const Epilogue& ep, hipStream_t s);
+
+// the product by tiles, from the codes (wc_gemm_codes.hip): k a multiple of 64, groups of 32, of whole 64 or the row, x as for
+// the dense product
+struct CodesArgs {
+    const void* x;
+    int64_t ldx, k;
+    const uint8_t* codes;
+    const void* scale;
+    const uint8_t* zp;
+    uint32_t groups, group_stages;  // per row; stages of 64 k per group (0: groups of 32)
+    uint64_t magic;                 // ceil(2^32 / group_stages)
+    RowMap rows;
+    Epilogue ep;
+    float* sums;  // [kz][rows][n], kz > 1
+    int kz;
+};
+struct CodesShape {
+    int fb, kz;  // tiles of 128 fb rows of x; blocks that share k
+    double us;
+};
+bool codes_fits(int mode, int64_t n, int64_t k, int64_t gs, const void* codes);
+CodesShape codes_plan(int mode, int64_t n, int64_t k, bool gated, int64_t rows, int64_t experts, bool grouped);
+int codes_launch(int dtype, int mode, int fb, const CodesArgs& a, hipStream_t s);
 
 }  // namespace wc

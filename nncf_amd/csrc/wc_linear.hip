@@ -380,42 +380,50 @@ int check_pointers(const char* what, const Weight& w) {
 }
 
 // What a call's workspace holds, one behind the other: the decompressed weight, the packed rows of x; and whether the product
-// runs on the codes themselves.
+// runs on the codes themselves, by strips for few rows (`few`) or by tiles (`tiles`): whichever way's estimate is the least.
 struct Need {
     size_t weight, pack;  // (the codes' product: the sums of blocks that share k in the weight's place)
-    bool few;
+    bool few, tiles;
     FewShape shape;
+    CodesShape codes;
     size_t total() const { return weight + pack; }
 };
-// The time of the other way, in the units of FewShape: the weight decompressed (2.6 bytes an element at 6 TB/s) and multiplied
+// The time of the dense way in us: the weight decompressed (2.6 bytes an element at 6 TB/s) and multiplied
 // by 128 x 128 or 256 x 256 tiles (1 and 1.6 us for 64 k of a round of blocks, the former 0.6 where half the blocks fill it).
-// 28672 x 8192: codes 144 us against 280 for 128 rows, 270 against 300 for 256, 520 against 365 for 512.
-int64_t dense_cost(const Weight& w, int64_t rows, bool grouped) {
+// 28672 x 8192 int4, us by strips, tiles and densely: 78, 106, 250 for 64 rows; 142, 102, 258 for 128; 270, 136, 270 for 256;
+// 537, 270, 315 for 512.  Eight experts of 4096 x 14336: 397, 253, 537 for 1200 rows, 814, 525, 615 for 3000, 1520, 1005, 909
+// for 6000.
+double dense_us(const Weight& w, int64_t rows, bool grouped) {
     auto blocks = [&](int64_t tile) { return ((w.n + tile - 1) / tile) * ((rows + tile - 1) / tile + (grouped ? (w.experts - 1) / 2 : 0)); };
     const int64_t small = blocks(128), large = blocks(256), steps = (w.k + 63) / 64;
     const double t128 = small <= 256 ? 0.6 : (double)((small + 511) / 512), t256 = 1.6 * (double)((large + 255) / 256);
-    const double us = (double)w.experts * (double)w.n * (double)w.k * 2.6 / 6.0e6 + (double)steps * (t128 < t256 ? t128 : t256) + 8.0;
-    return (int64_t)(us / 0.12);
+    return (double)w.experts * (double)w.n * (double)w.k * 2.6 / 6.0e6 + (double)steps * (t128 < t256 ? t128 : t256) + 8.0;
 }
 bool must_pack(const void* x, int64_t ldx, int64_t k, int64_t sources, bool gathered) {
     return k != padded(k) || ldx % 8 || ((uintptr_t)x & 15) || !dense_reaches(1, 32, ldx, sources, false, gathered);
 }
 Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, bool gathered, int64_t rows, bool gated, bool grouped) {
-    Need d{(size_t)(w.experts * w.n * padded(w.k)) * 2, 0, false, {}};
+    Need d{(size_t)(w.experts * w.n * padded(w.k)) * 2, 0, false, false, {}, {}};
     const bool copy = ldx % 8 || ((uintptr_t)x & 15);
     d.few = rows <= 1024 * w.experts && few_fits(w.mode, w.k, w.gs, w.codes, copy ? rows : sources, copy ? padded(w.k) : ldx);
+    double us = dense_us(w, rows, grouped);
     if (d.few) {
         d.shape = few_plan(w.mode, w.n, w.k, w.k / w.gs, gated, rows, w.experts, grouped);
-        d.few = d.shape.cost < dense_cost(w, rows, grouped);
+        d.few = (double)d.shape.cost * 0.12 < us;
+        if (d.few) us = (double)d.shape.cost * 0.12;
     }
-    if (d.few) {
-        d.weight = d.shape.kz > 1 ? (size_t)(d.shape.kz * rows * w.n + 3) / 4 * 16 : 0;
+    if (rows <= 4096 * w.experts && w.k == padded(w.k) && codes_fits(w.mode, w.n, w.k, w.gs, w.codes)) {
+        d.codes = codes_plan(w.mode, w.n, w.k, gated, rows, w.experts, grouped);
+        d.tiles = d.codes.us < us;
+        if (d.tiles) d.few = false;
     }
+    const int kz = d.few ? d.shape.kz : d.tiles ? d.codes.kz : 0;
+    if (kz) d.weight = kz > 1 ? (size_t)(kz * rows * w.n + 3) / 4 * 16 : 0;
     if (d.few ? copy : must_pack(x, ldx, w.k, sources, gathered)) d.pack = (size_t)(rows * padded(w.k)) * 2;
     return d;
 }
 Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
-    Need d{(size_t)(w.experts * w.k * padded(w.n)) * 2, 0, false, {}};
+    Need d{(size_t)(w.experts * w.k * padded(w.n)) * 2, 0, false, false, {}, {}};
     if (must_pack(dz, ldz, w.n, rows, false)) d.pack = (size_t)(rows * padded(w.n)) * 2;
     return d;
 }
@@ -438,16 +446,18 @@ int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* p
     return launch_status("linear: rows");
 }
 
+int out_of_range(int64_t n, int64_t k) {
+    set_error("linear: operands beyond the kernels' range (n=%lld k=%lld)", (long long)n, (long long)k);
+    return NNCF_AMD_ERR_UNSUPPORTED;
+}
+
 int run_dense(int dtype, const void* x, int64_t ldx, int64_t k, const void* w, RowMap rows, Epilogue ep, uint16_t* pack, hipStream_t s) {
     const int64_t kp = padded(k);
     if (must_pack(x, ldx, k, rows.sources, rows.slots != nullptr)) {
         const int st = pack_rows(x, ldx, k, rows, pack, s);
         if (st != NNCF_AMD_OK) return st;
     }
-    if (!dense_reaches(ep.n, kp, ldx, rows.sources, ep.act == kActSwiglu, rows.slots != nullptr)) {
-        set_error("linear: operands beyond the kernels' range (n=%lld k=%lld)", (long long)ep.n, (long long)k);
-        return NNCF_AMD_ERR_UNSUPPORTED;
-    }
+    if (!dense_reaches(ep.n, kp, ldx, rows.sources, ep.act == kActSwiglu, rows.slots != nullptr)) return out_of_range(ep.n, k);
     ep.vec = vec_of(ep);
     return dense_launch(dtype, DenseArgs{x, w, ldx, kp, rows, ep}, s);
 }
@@ -490,6 +500,20 @@ int forward(const char* what, const void* x, int dtype, int64_t ldx, const Weigh
         Epilogue e = ep;
         e.vec = vec_of(e);
         return few_launch(dtype, w.mode, FewArgs{x, ldx, w.codes, w.scale, w.zp, (uint32_t)w.k, groups, magic, scales8, map, e, (float*)ws}, need.shape, s);
+    }
+    if (need.tiles) {
+        RowMap map = rows;
+        if (need.pack) {
+            st = pack_rows(x, ldx, w.k, map, (uint16_t*)((char*)ws + need.weight), s);
+            if (st != NNCF_AMD_OK) return st;
+        }
+        if (!dense_reaches(w.n, w.k, ldx, map.sources, ep.act == kActSwiglu, map.slots != nullptr)) return out_of_range(w.n, w.k);
+        const uint32_t stages = w.gs % 64 ? 0 : (uint32_t)(w.gs / 64);
+        const uint64_t magic = stages ? (((uint64_t)1 << 32) + stages - 1) / stages : 0;
+        Epilogue e = ep;
+        e.vec = vec_of(e);
+        return codes_launch(dtype, w.mode, need.codes.fb,
+                            CodesArgs{x, ldx, w.k, w.codes, w.scale, w.zp, (uint32_t)(w.k / w.gs), stages, magic, map, e, (float*)ws, need.codes.kz}, s);
     }
     uint16_t* dense = (uint16_t*)ws;
     st = dtype == NNCF_AMD_BF16 ? dequant_rows<NNCF_AMD_BF16>(w, rows, dense, s) : dequant_rows<NNCF_AMD_F16>(w, rows, dense, s);

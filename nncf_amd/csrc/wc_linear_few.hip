@@ -297,7 +297,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
 
 // the blocks' sums over the parts of k, in their order, and the epilogue: a thread per 4 columns of a row
 template <int DT>
-__global__ __launch_bounds__(256) void k_few_join(const float* __restrict__ sums, int kz, RowMap rows, Epilogue ep) {
+__global__ __launch_bounds__(256) void k_join_sums(const float* __restrict__ sums, int kz, RowMap rows, Epilogue ep) {
     const int64_t width = ep.act == kActSwiglu ? ep.n / 2 : ep.n;
     const int64_t quads = (width + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     int64_t lo, end = rows.rows;
@@ -322,6 +322,17 @@ __global__ __launch_bounds__(256) void k_few_join(const float* __restrict__ sums
         }
     }
     finish4<DT>(ep, row, col, s, u);
+}
+
+int join_sums(int dtype, const float* sums, int kz, const RowMap& rows, const Epilogue& ep, hipStream_t s) {
+    const int64_t width = ep.act == kActSwiglu ? ep.n / 2 : ep.n, blocks = ((width + 3) / 4 * rows.rows + 255) / 256;
+    if (blocks > 0x7fffffff) {
+        set_error("linear: too many rows");
+        return NNCF_AMD_ERR_UNSUPPORTED;
+    }
+    if (dtype == NNCF_AMD_BF16) hipLaunchKernelGGL((k_join_sums<NNCF_AMD_BF16>), dim3((unsigned)blocks), dim3(256), 0, s, sums, kz, rows, ep);
+    else hipLaunchKernelGGL((k_join_sums<NNCF_AMD_F16>), dim3((unsigned)blocks), dim3(256), 0, s, sums, kz, rows, ep);
+    return launch_status("linear");
 }
 
 FewShape few_shape(int mode, int64_t k, int64_t groups, int wn, int wk, int kz, int rows, int tiles) {
@@ -417,13 +428,7 @@ int few_start(const FewArgs& a, const FewShape& sh, hipStream_t s) {
     hipLaunchKernelGGL((k_few_rows<MODE, DT, TT, XI>), grid, dim3(64 * sh.waves()), (size_t)sh.total(), s, a, sh);
     const int st = launch_status("linear");
     if (st != NNCF_AMD_OK || sh.kz == 1) return st;
-    const int64_t join = ((width + 3) / 4 * a.rows.rows + 255) / 256;
-    if (join > 0x7fffffff) {
-        set_error("linear: too many rows");
-        return NNCF_AMD_ERR_UNSUPPORTED;
-    }
-    hipLaunchKernelGGL((k_few_join<DT>), dim3((unsigned)join), dim3(256), 0, s, a.sums, sh.kz, a.rows, a.ep);
-    return launch_status("linear");
+    return join_sums(DT, a.sums, sh.kz, a.rows, a.ep, s);
 }
 
 template <int MODE, int DT>

@@ -1,0 +1,145 @@
+"""GPU: products with compressed weights at sizes where each way of computing them is taken (strips on the codes, tiles on the
+codes, a decompressed copy; with and without blocks that share k), against the plain product in 64 bits."""
+import pytest
+import torch
+
+from tests.linear_utils import FOUR, assert_within, make_weight, plain
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def _rows(m, k, dtype, seed):
+    g = torch.Generator(device="cpu").manual_seed(seed)
+    return torch.randn(m, k, generator=g).to(dtype).cuda()
+
+
+def _check(x, packed, dec, act=None, bias=None, residual=None):
+    from nncf_amd.linear import compressed_linear
+    got = compressed_linear(x, packed, dec, bias=bias, activation=act, residual=residual)
+    y, by = plain(x, dec(packed), bias, act, residual)
+    assert_within(got, y, by, (tuple(x.shape), act))
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 16, 33, 64, 65, 97, 128, 129, 200, 257, 520, 900])
+@pytest.mark.parametrize("mode,gs,n,k", [("int4_sym", 128, 1000, 4096), ("int4_asym", 64, 518, 4160), ("nf4", 32, 640, 2080),
+                                         ("mxfp4", 32, 1024, 2112), ("int8_asym", -1, 777, 2048), ("int8_sym", -1, 512, 4032),
+                                         ("int4_asym", -1, 260, 4096), ("nf4", 64, 130, 8192), ("int4_asym", 32, 131, 2112)])
+def test_every_way_by_rows(mode, gs, n, k, m, dtype):
+    packed, dec = make_weight(mode, gs, (n, k), dtype, seed=m + n)
+    _check(_rows(m, k, dtype, m), packed, dec)
+
+
+@pytest.mark.parametrize("m", [3, 90, 200, 700])
+@pytest.mark.parametrize("act", ["swiglu", "gelu", "silu", None])
+@pytest.mark.parametrize("mode,gs,n,k", [("int4_asym", 128, 1032, 2048), ("mxfp4", 32, 518, 4096), ("int8_sym", -1, 640, 2048)])
+def test_epilogue_where_blocks_share_k(mode, gs, n, k, act, m):
+    dtype = torch.bfloat16
+    packed, dec = make_weight(mode, gs, (n, k), dtype, seed=m)
+    width = n // 2 if act == "swiglu" else n
+    g = torch.Generator(device="cpu").manual_seed(m)
+    bias, residual = torch.randn(n, generator=g).to(dtype).cuda(), torch.randn(m, width, generator=g).to(dtype).cuda()
+    _check(_rows(m, k, dtype, m) * 0.1, packed, dec, act, bias, residual)
+
+
+@pytest.mark.parametrize("act", ["swiglu", "gelu", None])
+@pytest.mark.parametrize("m", [40, 130, 300])
+@pytest.mark.parametrize("mode,gs,n,k", [("int4_sym", 64, 20000, 256), ("nf4", 32, 17666, 192), ("int8_asym", -1, 18000, 320)])
+def test_tiles_that_fill_the_device(mode, gs, n, k, m, act):
+    """Tiles enough that no blocks share k: the epilogue in the product's own kernel, the last tile ragged."""
+    dtype = torch.float16
+    packed, dec = make_weight(mode, gs, (n, k), dtype, seed=m)
+    width = n // 2 if act == "swiglu" else n
+    g = torch.Generator(device="cpu").manual_seed(m)
+    bias, residual = torch.randn(n, generator=g).to(dtype).cuda(), torch.randn(m, width, generator=g).to(dtype).cuda()
+    _check(_rows(m, k, dtype, m) * 0.1, packed, dec, act, bias, residual)
+
+
+@pytest.mark.parametrize("m", [2, 100, 300])
+def test_strided_and_misaligned_rows(m):
+    """Rows further apart than they are long, rows that no vector load may touch, and results into the middle of a matrix."""
+    from nncf_amd.linear import compressed_linear
+    packed, dec = make_weight("int4_sym", 128, (1000, 4096), torch.bfloat16, seed=1)
+    x = _rows(m, 4096, torch.bfloat16, m)
+    want = compressed_linear(x, packed, dec)
+    y, by = plain(x, dec(packed))
+    assert_within(want, y, by)
+    for pad, shift in ((8, 0), (64, 8), (3, 1), (5, 0)):
+        wide = torch.empty(m, 4096 + pad, dtype=x.dtype, device="cuda")
+        wide[:, shift:shift + 4096] = x
+        assert torch.equal(compressed_linear(wide[:, shift:shift + 4096], packed, dec), want)
+
+
+@pytest.mark.parametrize("m", [97, 257])
+def test_train_where_the_forward_pass_runs_on_the_codes(m):
+    """z is kept by the kernel that joins the parts of k (or by the tiles' own): the gradients see it."""
+    from nncf_amd.linear import compressed_linear
+    dtype, n, k = torch.bfloat16, 520, 2048
+    for mode, act in (("int4_asym", "gelu"), ("nf4", "swiglu"), ("int8_sym", "silu")):
+        packed, dec = make_weight(mode, -1 if mode == "int8_sym" else 64, (n, k), dtype, seed=m)
+        x = (_rows(m, k, dtype, m) * 0.1).requires_grad_()
+        bias = torch.randn(n, generator=torch.Generator().manual_seed(m)).to(dtype).cuda().requires_grad_()
+        y = compressed_linear(x, packed, dec, bias=bias, activation=act)
+        dy = _rows(m, y.shape[-1], dtype, m + 1)
+        y.backward(dy)
+        ref = plain(x.detach(), dec(packed), bias.detach(), act, None, dy)
+        assert_within(y.detach(), ref[0], ref[1], "y")
+        assert_within(x.grad, ref[2], ref[3], "dx")
+        assert_within(bias.grad, ref[4], ref[5], "dbias")
+
+
+@pytest.mark.parametrize("mode", FOUR + ("int8_asym",))
+@pytest.mark.parametrize("skew", ["even", "one", "edges"])
+@pytest.mark.parametrize("gather,act", [(True, None), (False, "swiglu")])
+def test_experts_on_tiles(mode, skew, gather, act):
+    """Groups of 0, 1, 127, 128, 129 and several hundred rows over tiles of 128 and 256, rows behind the last group."""
+    from nncf_amd.experts import expert_linear, route_experts
+    dtype, experts, n, k = torch.bfloat16, 6, 516, 1024
+    sizes = {"even": [110] * 6, "one": [0, 0, 640, 0, 3, 0], "edges": [127, 128, 129, 0, 1, 257]}[skew]
+    tokens = sum(sizes) + 9
+    logits = torch.full((tokens, experts), -8.0)
+    at = 0
+    for e, size in enumerate(sizes):
+        logits[at:at + size, e] = 1.0
+        at += size
+    perm = torch.randperm(tokens, generator=torch.Generator().manual_seed(5))
+    mask = torch.arange(tokens) < at
+    r = route_experts(logits[perm].cuda(), 1, token_mask=mask[perm].cuda())
+    off = r.offsets.tolist()
+    assert [b - a for a, b in zip(off, off[1:])] == sizes
+    packed, dec = make_weight(mode, -1 if mode == "int8_asym" else 32, (experts, n, k), dtype, seed=7)
+    w = dec(packed)
+    x = _rows(tokens, k, dtype, 3)
+    y = expert_linear(x, packed, dec, r, gather=gather, activation=act)
+    source = r.slots.long() if gather else torch.arange(tokens, device="cuda")
+    for e in range(experts):
+        if off[e] == off[e + 1]:
+            continue
+        want, by = plain(x[source[off[e]:off[e + 1]]], w[e], None, act)
+        assert_within(y[off[e]:off[e + 1]], want, by, (e, sizes[e]))
+    assert not y[off[-1]:].any()
+
+
+def test_offsets_beyond_31_bits():
+    """A stack whose codes, values and parameters lie more than 2^31 bytes and elements behind its start."""
+    from nncf_amd import decompressors as D
+    from nncf_amd.experts import expert_linear, route_experts
+    dtype, experts, n, k = torch.bfloat16, 80, 8192, 8192
+    codes = torch.randint(0, 256, (experts * n * k // 2, 1), dtype=torch.uint8, device="cuda")
+    scale = (torch.rand(experts, n, k // 64, 1, device="cuda") * 0.02 + 0.002).half()
+    dec = D.INT4SymmetricWeightsDecompressor(scale, compressed_weight_shape=(experts, n, k // 64, 64), result_shape=(experts, n, k),
+                                             result_dtype=dtype)
+    one = D.INT4SymmetricWeightsDecompressor(scale[-1], compressed_weight_shape=(n, k // 64, 64), result_shape=(n, k), result_dtype=dtype)
+    w = one(codes.reshape(experts, -1)[-1].reshape(-1, 1))
+    for tokens in (2, 150):
+        logits = torch.zeros(tokens, experts, device="cuda")
+        logits[:, -1] = 1
+        x = _rows(tokens, k, dtype, tokens)
+        y = expert_linear(x, codes, dec, route_experts(logits, 1))
+        want, by = plain(x, w[:512])
+        assert_within(y[:, :512], want, by)
+        want, by = plain(x, w[-512:])
+        assert_within(y[:, -512:], want, by)
