@@ -416,8 +416,8 @@ int nncf_amd_gptq_dequant8(const int32_t* qweight, const int32_t* qzeros, const 
  *   activation : 0 none, 1 relu, 2 gelu (erf), 3 gelu (tanh), 4 silu, 5 swiglu: rows [0, n / 2) of W are the gate, y has n / 2
  *                columns silu(gate) * up
  *   residual   : [m, width] in x's type, rows ldr apart, nullable
- *   y          : [m, width], rows ldy apart;  z : [m, n] nullable, the sums with their bias in x's type (what the gradient of
- *                the activation needs)
+ *   y          : [m, width], rows ldy apart;  slope : [m, n] fp32, nullable, the activation's derivatives at the sums
+ *                (swiglu: up * silu'(gate) and silu(gate)), which nncf_amd_activation_grad takes
  *   workspace  : nncf_amd_compressed_linear_workspace bytes, aligned to 16 (0: none needed)
  */
 size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t m, int64_t n, int64_t k,
@@ -425,7 +425,7 @@ size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ldx, int64_t 
 int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes,
                                int mode, int64_t group_size, const void* scale, const uint8_t* zero_point,
                                const void* bias, int activation, const void* residual, int64_t ldr, void* y, int64_t ldy,
-                               void* z, void* workspace, size_t workspace_bytes, void* stream);
+                               float* slope, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * The same for a stack of experts' weights [experts, n, k] and rows in the order of their experts: expert e owns the rows
  * [offsets[e], offsets[e + 1]) of y (int32 [experts + 1], on the device); rows behind offsets[experts] get zeros.
@@ -438,7 +438,7 @@ size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, int64_t sour
 int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int64_t sources, const int32_t* slots, int64_t topk,
                            const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k, const void* codes,
                            int mode, int64_t group_size, const void* scale, const uint8_t* zero_point, int activation,
-                           void* y, int64_t ldy, void* z, void* workspace, size_t workspace_bytes, void* stream);
+                           void* y, int64_t ldy, float* slope, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * dx = dz W for either (offsets == NULL: experts is 1), dz [rows, n] in the activations' type, rows ldz apart; dx [rows, k] in
  * that type or fp32 (dx_is_f32), rows ldx apart.
@@ -450,12 +450,12 @@ int nncf_amd_linear_grad_input(const void* dz, int dtype, int64_t ldz, const int
                                const void* scale, const uint8_t* zero_point, void* dx, int64_t ldx, int dx_is_f32,
                                void* workspace, size_t workspace_bytes, void* stream);
 /*
- * dz = dy * act'(z) [m, n] in the activations' type with rows ldz apart (the columns behind n become zero), nullable; and
- * dbias [n] = the sums of dz over the rows, in fp32 and in a fixed order, rounded once; nullable.  z may be NULL without an
+ * dz = dy * slope [m, n] in the activations' type with rows ldz apart (the columns behind n become zero), nullable; and
+ * dbias [n] = the sums of dz over the rows, in fp32 and in a fixed order, rounded once; nullable.  slope may be NULL without an
  * activation.  workspace: only for dbias.
  */
 size_t nncf_amd_activation_grad_workspace(int64_t m, int64_t n);
-int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, const void* z, int64_t m, int64_t n, int activation,
+int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, const float* slope, int64_t m, int64_t n, int activation,
                              void* dz, int64_t ldz, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 /*
  * Routing of tokens to experts: the topk largest logits of every row of [tokens, experts] (fp32 / fp16 / bf16, rows ldl

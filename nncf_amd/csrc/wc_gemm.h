@@ -86,9 +86,9 @@ __device__ __forceinline__ void zero_rows(const RowMap& rows, const Epilogue& e,
         for (int64_t c = col + threadIdx.x; c < end; c += THREADS) {
             if (e.y32) ((float*)e.y)[r * e.ldy + c] = 0.0f;
             else ((uint16_t*)e.y)[r * e.ldy + c] = 0;
-            if (e.z) {
-                ((uint16_t*)e.z)[r * e.n + c] = 0;
-                if (gated) ((uint16_t*)e.z)[r * e.n + width + c] = 0;
+            if (e.slope) {
+                e.slope[r * e.n + c] = 0.0f;
+                if (gated) e.slope[r * e.n + width + c] = 0.0f;
             }
         }
 }
@@ -126,7 +126,7 @@ __device__ __forceinline__ void finish_rows(const Epilogue& e, const float* tile
             const uint32_t r = (t0 + t) * ROWS + r0;
             const int64_t row = row0 + r;
             const float* at = tile + r * PITCH + lane % LANES * 8;
-            float z[8], u[GATED ? 8 : 1], v[8];
+            float z[8], u[GATED ? 8 : 1] = {}, v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 z[i] = at[i] + bz[i];
@@ -148,10 +148,13 @@ __device__ __forceinline__ void finish_rows(const Epilogue& e, const float* tile
                 for (int j = 0; j < 4; ++j) v[2 * j] += to_f32<DT>((uint16_t)res[t][j]), v[2 * j + 1] += to_f32<DT>((uint16_t)(res[t][j] >> 16));
             }
             *(halves8*)((uint16_t*)e.y + row * e.ldy + col) = pack(v);
-            if (e.z) {
-                uint16_t* z_at = (uint16_t*)e.z + row * e.n + col;
-                *(halves8*)z_at = pack(z);
-                if constexpr (GATED) *(halves8*)(z_at + width) = pack(u);
+            if (e.slope) {
+                float* to = e.slope + row * e.n + col;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) slopes(ACT, z[i], u[GATED ? i : 0]);
+                *(f32x4*)to = f32x4{z[0], z[1], z[2], z[3]}, *(f32x4*)(to + 4) = f32x4{z[4], z[5], z[6], z[7]};
+                if constexpr (GATED)
+                    *(f32x4*)(to + width) = f32x4{u[0], u[1], u[2], u[3]}, *(f32x4*)(to + width + 4) = f32x4{u[4], u[5], u[6], u[7]};
             }
         }
     }

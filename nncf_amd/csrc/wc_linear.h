@@ -1,5 +1,5 @@
-// wc_linear.h -- shared by the kernels that multiply activations by compressed weights (wc_linear.hip, wc_gemm_nt.hip,
-// wc_experts.hip).
+// wc_linear.h -- shared by the kernels that multiply activations by compressed weights (wc_linear.hip, wc_linear_few.hip,
+// wc_gemm_nt.hip, wc_gemm_codes.hip, wc_experts.hip).
 //
 // The operator:  y[m, :] = act(x[m, :] . W^T + bias) + residual[m, :],  W [n, k] given as codes, scales and zero points.
 // W is the VALUE OF THE DECOMPRESSOR in the activations' type (wc_decompress.hip), bit for bit:
@@ -240,12 +240,20 @@ struct Epilogue {
     const void* bias;      // [n] or null
     const void* residual;  // [rows, width] or null
     void* y;               // [rows, width]
-    void* z;               // [rows, n] or null: the sums with their bias, for the gradient of the activation
+    float* slope;          // [rows, n] or null: what the gradient of a row's sums takes dy times (`slopes`)
     int64_t ldr, ldy, n;   // n: rows of the weight; swiglu: gate rows first, width = n / 2
     int act;
     int y32;               // y is fp32 (gradients that are summed over rows afterwards)
-    int vec;               // 4 consecutive columns may be stored as 8 bytes (y, residual, z and their row strides allow it)
+    int vec;               // 4 consecutive columns may be stored at once (y, residual, slope and their row strides allow it)
 };
+
+// The activation's derivative in place of the sum z (swiglu: those of both halves, z and u, in their places).  They are kept in
+// fp32: in 16 bits, they or the sums, they double the rounding error of the bias' gradient (bf16: 0.0031 for 0.0017 of its norm).
+__device__ __forceinline__ void slopes(int act, float& z, float& u) {
+    const float at = z;
+    if (act == kActSwiglu) z = u * activate_grad(kActSilu, at), u = at * sigmoid_f(at);
+    else z = activate_grad(act, at);
+}
 
 // up to four consecutive columns of one row; `up` only for swiglu (a: the gate's sums, b: the other half's)
 template <int DT>
@@ -265,10 +273,11 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
         }
         __builtin_amdgcn_sched_barrier(0);  // one after the other: side by side their exponentials need the most registers
         v[i] = e.act == kActSwiglu ? z[i] * sigmoid_f(z[i]) * u[i] : activate(e.act, z[i]);
+        if (e.slope) slopes(e.act, z[i], u[i]);
     }
     uint16_t* y = (uint16_t*)e.y + row * e.ldy + col;
     const uint16_t* res = e.residual ? (const uint16_t*)e.residual + row * e.ldr + col : nullptr;
-    uint16_t* zo = e.z ? (uint16_t*)e.z + row * e.n + col : nullptr;
+    float* so = e.slope ? e.slope + row * e.n + col : nullptr;
     if (e.y32) {
         float* y32 = (float*)e.y + row * e.ldy + col;
         if (e.vec && cnt == 4) *(f32x4*)y32 = f32x4{v[0], v[1], v[2], v[3]};
@@ -283,9 +292,9 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
             v[2] += to_f32<DT>((uint16_t)r.y), v[3] += to_f32<DT>((uint16_t)(r.y >> 16));
         }
         *(u32v2*)y = u32v2{pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3])};
-        if (zo) {
-            *(u32v2*)zo = u32v2{pair_of<DT>(z[0], z[1]), pair_of<DT>(z[2], z[3])};
-            if (e.act == kActSwiglu) *(u32v2*)(zo + width) = u32v2{pair_of<DT>(u[0], u[1]), pair_of<DT>(u[2], u[3])};
+        if (so) {
+            *(f32x4*)so = f32x4{z[0], z[1], z[2], z[3]};
+            if (e.act == kActSwiglu) *(f32x4*)(so + width) = f32x4{u[0], u[1], u[2], u[3]};
         }
         return;
     }
@@ -294,14 +303,15 @@ __device__ __forceinline__ void finish4(const Epilogue& e, int64_t row, int64_t 
         if (i >= cnt) break;
         if (res) v[i] += to_f32<DT>(res[i]);
         y[i] = from_f32<DT>(v[i]);
-        if (zo) {
-            zo[i] = from_f32<DT>(z[i]);
-            if (e.act == kActSwiglu) zo[width + i] = from_f32<DT>(u[i]);
+        if (so) {
+            so[i] = z[i];
+            if (e.act == kActSwiglu) so[width + i] = u[i];
         }
     }
 }
 
-// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 64, 192 at least, and 16-byte rows, w [experts * n, k]
+// the product of dense operands (wc_gemm_nt.hip): x [sources, ldx] with k a multiple of 64, 192 at least, and 16-byte rows,
+// w [experts * n, k]
 struct DenseArgs {
     const void* x;
     const void* w;
@@ -313,7 +323,8 @@ struct DenseArgs {
 bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gated, bool gathered);
 int dense_launch(int dtype, const DenseArgs& a, hipStream_t s);
 
-// the product for few rows per group, from the codes (wc_linear_few.hip): rows of whole 32 k, groups of 32, of whole 64 or the row, 16-byte rows of x
+// the product for few rows per group, from the codes (wc_linear_few.hip): rows of whole 32 k, groups of 32, of whole 64 or the
+// row, 16-byte rows of x
 struct FewArgs {
     const void* x;
     int64_t ldx;

@@ -12,9 +12,10 @@ namespace wc {
 constexpr int64_t padded(int64_t v) { return v <= 192 ? 192 : (v + 63) / 64 * 64; }
 
 // ---------------------------------------------------------------------------------- weight -> dense rows of the workspace
-// [experts * n, kp], kp = k rounded up to 64 (192 at least), the tail zero.  Bound by the bytes (0.5-1 read, 2 written per weight).  `lanes` (a
-// power of two) threads follow a row, 8 weights each; a thread takes the same place of kDequantRows rows, whose reads are
-// requested together and whose addresses are a scalar apart.  An expert without rows is left out.
+// [experts * n, kp], kp = k rounded up to 64 (192 at least), the tail zero.  Bound by the bytes (0.5-1 read, 2 written per
+// weight).  `lanes` (a power of two) threads follow a row, 8 weights each; a thread takes the same place of kDequantRows rows,
+// whose reads are requested together and whose addresses are a scalar apart.  An expert without rows is left out.
+// 28672 x 8192 int4: 101 us, 5.9 TB/s; eight NF4 experts of 28672 x 4096, groups of 32: 405 us, 6.0 TB/s.
 constexpr int kDequantRows = 4;
 template <int MODE, int DT>
 __global__ __launch_bounds__(256) void k_dequant_rows(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
@@ -89,8 +90,9 @@ __global__ __launch_bounds__(256) void k_dequant_rows_any(const uint8_t* __restr
 }
 
 // ------------------------------------------------------------------------- weight -> its transpose, for the gradient of x
-// [experts, k, np], np = n rounded up to 64 (192 at least), the tail zero: tiles of 64 x 64 turned round in LDS as pairs of neighbouring n
-// (rows padded by 4 bytes so that the columns that are written fall on different banks).
+// [experts, k, np], np = n rounded up to 64 (192 at least), the tail zero: tiles of 64 x 64 turned round in LDS as pairs of
+// neighbouring n (rows padded by 4 bytes so that the columns that are written fall on different banks).  Bound by the bytes:
+// eight int4 weights of 4096 x 14336 in 292 us, 4.0 TB/s (one tile at a time 340: its reads of 32 bytes a row wait alone).
 constexpr int kTurns = 4;
 template <int MODE, int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_dequant_transposed(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
@@ -172,13 +174,14 @@ __global__ __launch_bounds__(256) void k_pack_rows(const uint16_t* __restrict__ 
 }
 
 // ------------------------------------------------------------------------------------- gradient of the epilogue's activation
-// dz = dy * act'(z) (swiglu: both halves), written with row stride ldz and zeros behind n; and the sums of dz's fp32 values
+// dz = dy * slope (swiglu: both halves), written with row stride ldz and zeros behind n; and the sums of dz's fp32 values
 // over chunks of 32 rows, which k_sum_chunks adds up in order (no atomics: the result does not depend on the schedule).
 // dz is rounded to the activations' type because the product that takes it reads 16-bit operands.
-// A thread takes VEC consecutive columns; the chunk's rows are dealt to 4 waves whose sums meet in LDS, wave 0 first.
+// A thread takes VEC consecutive columns; the chunk's rows are dealt to 4 waves whose sums meet in LDS, wave 0 first.  Bound by
+// the bytes, 8 an element: 2047 x 4096 in 17 us.
 constexpr int kChunkRows = 32;
 template <int DT, int VEC>
-__global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restrict__ dy, int64_t ldd, const uint16_t* __restrict__ z,
+__global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restrict__ dy, int64_t ldd, const float* __restrict__ slope,
                                                          int64_t m, int64_t n, int act, uint16_t* __restrict__ dz, int64_t ldz,
                                                          float* __restrict__ sums) {
     __shared__ float part[3][2 * VEC][64];
@@ -198,6 +201,14 @@ __global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restr
             v[0] = to_f32<DT>(*p);
         }
     };
+    auto read32 = [&](const float* p, float* v) {
+        if constexpr (VEC == 4) {
+            const f32x4 w = *(const f32x4*)p;
+            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+        } else {
+            v[0] = *p;
+        }
+    };
     auto write = [&](uint16_t* p, const float* v) {
         if constexpr (VEC == 4) *(u32v2*)p = u32v2{pair_of<DT>(v[0], v[1]), pair_of<DT>(v[2], v[3])};
         else *p = from_f32<DT>(v[0]);
@@ -208,21 +219,21 @@ __global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restr
             float g[VEC], a[VEC];
             read(dy + r * ldd + c, g);
             if (act == kActSwiglu) {
-                float zg[VEC], zu[VEC], b[VEC];
-                read(z + r * n + c, zg);
-                read(z + r * n + width + c, zu);
+                float sg[VEC], su[VEC], b[VEC];
+                read32(slope + r * n + c, sg);
+                read32(slope + r * n + width + c, su);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    a[i] = g[i] * zu[i] * activate_grad(kActSilu, zg[i]);
-                    b[i] = g[i] * zg[i] * sigmoid_f(zg[i]);
+                    a[i] = g[i] * sg[i];
+                    b[i] = g[i] * su[i];
                     s1[i] += b[i];
                 }
                 if (dz) write(dz + r * ldz + width + c, b);
             } else if (act != kActNone) {
                 float v[VEC];
-                read(z + r * n + c, v);
+                read32(slope + r * n + c, v);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) a[i] = g[i] * activate_grad(act, v[i]);
+                for (int i = 0; i < VEC; ++i) a[i] = g[i] * v[i];
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) a[i] = g[i];
@@ -430,9 +441,9 @@ Need backward_need(const Weight& w, const void* dz, int64_t ldz, int64_t rows) {
 
 int vec_of(const Epilogue& e) {
     const int64_t width = e.act == kActSwiglu ? e.n / 2 : e.n;
-    uintptr_t bits = (uintptr_t)e.y | (uintptr_t)e.z | (uintptr_t)e.residual;
+    uintptr_t bits = (uintptr_t)e.y | (uintptr_t)e.residual;
     if (e.y32 && ((uintptr_t)e.y & 15)) return 0;
-    return (bits & 7) == 0 && e.ldy % 4 == 0 && (!e.residual || e.ldr % 4 == 0) && (!e.z || width % 4 == 0);
+    return (bits & 7) == 0 && ((uintptr_t)e.slope & 15) == 0 && e.ldy % 4 == 0 && (!e.residual || e.ldr % 4 == 0) && (!e.slope || width % 4 == 0);
 }
 
 int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* pack, hipStream_t s) {
@@ -568,7 +579,7 @@ extern "C" size_t nncf_amd_compressed_linear_workspace(const void* x, int64_t ld
 
 extern "C" int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, const void* codes, int mode,
                                           int64_t group_size, const void* scale, const uint8_t* zero_point, const void* bias, int activation,
-                                          const void* residual, int64_t ldr, void* y, int64_t ldy, void* z, void* workspace,
+                                          const void* residual, int64_t ldr, void* y, int64_t ldy, float* slope, void* workspace,
                                           size_t workspace_bytes, void* stream) {
     using namespace wc;
     const Weight w{(const uint8_t*)codes, scale, zero_point, mode, n, k, group_size == -1 ? k : group_size, 1};
@@ -580,7 +591,7 @@ extern "C" int nncf_amd_compressed_linear(const void* x, int dtype, int64_t ldx,
     }
     const RowMap rows{nullptr, nullptr, 1, 1, m, m};
     Epilogue ep{};
-    ep.bias = bias, ep.residual = residual, ep.y = y, ep.z = z, ep.ldr = ldr, ep.ldy = ldy, ep.n = n, ep.act = activation;
+    ep.bias = bias, ep.residual = residual, ep.y = y, ep.slope = slope, ep.ldr = ldr, ep.ldy = ldy, ep.n = n, ep.act = activation;
     return forward("compressed_linear", x, dtype, ldx, w, rows, ep, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -596,7 +607,7 @@ extern "C" size_t nncf_amd_expert_linear_workspace(const void* x, int64_t ldx, i
 extern "C" int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int64_t sources, const int32_t* slots, int64_t topk,
                                       const int32_t* offsets, int64_t experts, int64_t rows, int64_t n, int64_t k, const void* codes,
                                       int mode, int64_t group_size, const void* scale, const uint8_t* zero_point, int activation, void* y,
-                                      int64_t ldy, void* z, void* workspace, size_t workspace_bytes, void* stream) {
+                                      int64_t ldy, float* slope, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace wc;
     const Weight w{(const uint8_t*)codes, scale, zero_point, mode, n, k, group_size == -1 ? k : group_size, experts};
     int st = check_weight("expert_linear", dtype, w);
@@ -604,7 +615,7 @@ extern "C" int nncf_amd_expert_linear(const void* x, int dtype, int64_t ldx, int
     if (st != NNCF_AMD_OK) return st;
     const RowMap map{offsets, slots, (int32_t)experts, (int32_t)topk, rows, sources};
     Epilogue ep{};
-    ep.y = y, ep.z = z, ep.ldy = ldy, ep.n = n, ep.act = activation;
+    ep.y = y, ep.slope = slope, ep.ldy = ldy, ep.n = n, ep.act = activation;
     return forward("expert_linear", x, dtype, ldx, w, map, ep, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
@@ -635,7 +646,7 @@ extern "C" size_t nncf_amd_activation_grad_workspace(int64_t m, int64_t n) {
     return m < 1 || n < 1 ? 0 : (size_t)((m + wc::kChunkRows - 1) / wc::kChunkRows) * (size_t)n * 4;
 }
 
-extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, const void* z, int64_t m, int64_t n, int activation, void* dz,
+extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, const float* slope, int64_t m, int64_t n, int activation, void* dz,
                                         int64_t ldz, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     using namespace wc;
     if (dtype != NNCF_AMD_F16 && dtype != NNCF_AMD_BF16) {
@@ -649,9 +660,10 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
     const int64_t width = activation == kActSwiglu ? n / 2 : n;
     const int64_t chunks = (m + kChunkRows - 1) / kChunkRows;
     // four columns a thread where every row of every operand allows 8-byte accesses
-    const bool wide = width % 4 == 0 && n % 4 == 0 && ldd % 4 == 0 && (!dz || ldz % 4 == 0) && (((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz) & 7) == 0;
+    const bool wide = width % 4 == 0 && n % 4 == 0 && ldd % 4 == 0 && (!dz || ldz % 4 == 0) && (((uintptr_t)dy | (uintptr_t)dz) & 7) == 0 &&
+                      ((uintptr_t)slope & 15) == 0;
     const int64_t per = wide ? 256 : 64, blocks = (width + (dz ? ldz - n : 0) + per - 1) / per;
-    if (m > 0 && (!dy || ldd < width || (activation != kActNone && !z) || (dz && ldz < n))) {
+    if (m > 0 && (!dy || ldd < width || (activation != kActNone && !slope) || (dz && ldz < n))) {
         set_error("activation_grad: null or overlapping rows (ldd=%lld ldz=%lld)", (long long)ldd, (long long)ldz);
         return NNCF_AMD_ERR_BAD_ARG;
     }
@@ -668,7 +680,7 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
     if (m > 0 && (dz || dbias)) {
         const dim3 grid((unsigned)blocks, (unsigned)chunks);
 #define GO(DT, VEC)                                                                                                              \
-    hipLaunchKernelGGL((k_activation_grad<DT, VEC>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, (const uint16_t*)z, m, n, \
+    hipLaunchKernelGGL((k_activation_grad<DT, VEC>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, slope, m, n, \
                        activation, (uint16_t*)dz, ldz, sums)
         if (dtype == NNCF_AMD_BF16) {
             if (wide) GO(NNCF_AMD_BF16, 4);

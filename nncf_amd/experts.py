@@ -135,36 +135,36 @@ def _check_routing(routing: ExpertRouting, device, what: str, experts: Optional[
     return tokens, top_k
 
 
-def _expert_forward(x, w: PackedWeight, slots, offsets, rows: int, top_k: int, gather: bool, act: int, width: int, want_z: bool):
+def _expert_forward(x, w: PackedWeight, slots, offsets, rows: int, top_k: int, gather: bool, act: int, width: int, want_slope: bool):
     src, ldx = rows_of(x, w.k)
     y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
-    z = torch.empty((rows, w.n), dtype=x.dtype, device=x.device) if want_z else None
+    slope = torch.empty((rows, w.n), dtype=torch.float32, device=x.device) if want_slope else None
     L = _lib.lib()
     ws = workspace_of(L.nncf_amd_expert_linear_workspace(ptr(src), ldx, src.shape[0], int(gather), rows, w.n, w.k, ptr(w.codes), w.mode,
                                                          w.group_size, w.experts, act), x.device)
     _lib.check(L.nncf_amd_expert_linear(ptr(src), _DTYPES[x.dtype], ldx, src.shape[0], ptr(slots) if gather else None, top_k,
                                         ptr(offsets), w.experts, rows, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
-                                        ptr(w.scale), ptr(w.zero_point), act, ptr(y), width, ptr(z), ptr(ws),
+                                        ptr(w.scale), ptr(w.zero_point), act, ptr(y), width, ptr(slope), ptr(ws),
                                         0 if ws is None else ws.numel(), _lib.raw_stream(x)))
-    return y, z
+    return y, slope
 
 
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, slots, offsets, places, gather, act, width):
         with _lib.on_device_of(x):
-            y, z = _expert_forward(x, w, slots, offsets, slots.shape[0], places.shape[1], gather, act, width, act != 0)
-        ctx.save_for_backward(z, w.codes, w.scale, w.zero_point, offsets, places)
+            y, slope = _expert_forward(x, w, slots, offsets, slots.shape[0], places.shape[1], gather, act, width, act != 0)
+        ctx.save_for_backward(slope, w.codes, w.scale, w.zero_point, offsets, places)
         ctx.weight, ctx.act, ctx.dtype, ctx.gather = w[3:], act, x.dtype, gather
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        z, codes, scale, zp, offsets, places = ctx.saved_tensors
+        slope, codes, scale, zp, offsets, places = ctx.saved_tensors
         w = PackedWeight(codes, scale, zp, *ctx.weight)
         with _lib.on_device_of(dy):
-            dz, ldz, _ = activation_grad(dy, z, w.n, ctx.act, ctx.dtype, True, False)
+            dz, ldz, _ = activation_grad(dy, slope, w.n, ctx.act, ctx.dtype, True, False)
             # a token's rows are added up in fp32 and rounded once
             dx = grad_input(dz, ldz, w, offsets, ctx.dtype, fp32=ctx.gather)
             if ctx.gather:

@@ -133,8 +133,8 @@ def workspace_of(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def activation_grad(dy: torch.Tensor, z: Optional[torch.Tensor], n: int, act: int, dtype: torch.dtype, want_dz: bool, want_dbias: bool):
-    """(dz, its row stride, dbias) of the epilogue: dz = dy * act'(z), padded to whole steps of the product that follows."""
+def activation_grad(dy: torch.Tensor, slope: Optional[torch.Tensor], n: int, act: int, dtype: torch.dtype, want_dz: bool, want_dbias: bool):
+    """(dz, its row stride, dbias) of the epilogue: dz = dy * slope, padded to whole steps of the product that follows."""
     width = n // 2 if act == _SWIGLU else n
     dy, ldd = rows_of(dy, width)
     m = dy.shape[0]
@@ -146,7 +146,7 @@ def activation_grad(dy: torch.Tensor, z: Optional[torch.Tensor], n: int, act: in
     dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
     dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
     ws = workspace_of(L.nncf_amd_activation_grad_workspace(m, n) if want_dbias else 0, dy.device)
-    _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(z), m, n, act, ptr(dz), ldz, ptr(dbias),
+    _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(slope), m, n, act, ptr(dz), ldz, ptr(dbias),
                                           ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dy)))
     return (dz, ldz, dbias) if copies else (dy, ldd, dbias)
 
@@ -163,42 +163,42 @@ def grad_input(dz: torch.Tensor, ldz: int, w: PackedWeight, offsets: Optional[to
     return dx
 
 
-def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_z: bool):
-    """(y [m, width], z [m, n] or None) of rows x [..., k]."""
+def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_slope: bool):
+    """(y [m, width], slope [m, n] or None) of rows x [..., k]."""
     rows, ldx = rows_of(x, w.k)
     m = rows.shape[0]
     y = torch.empty((m, width), dtype=x.dtype, device=x.device)
-    z = torch.empty((m, w.n), dtype=x.dtype, device=x.device) if want_z else None
+    slope = torch.empty((m, w.n), dtype=torch.float32, device=x.device) if want_slope else None
     res, ldr = (None, 0) if residual is None else rows_of(residual, width)
     L = _lib.lib()
     ws = workspace_of(L.nncf_amd_compressed_linear_workspace(ptr(rows), ldx, m, w.n, w.k, ptr(w.codes), w.mode,
                                                              w.group_size, act), x.device)
     _lib.check(L.nncf_amd_compressed_linear(ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
                                             ptr(w.scale), ptr(w.zero_point), ptr(bias), act, ptr(res), ldr,
-                                            ptr(y), width, ptr(z), ptr(ws), 0 if ws is None else ws.numel(),
+                                            ptr(y), width, ptr(slope), ptr(ws), 0 if ws is None else ws.numel(),
                                             _lib.raw_stream(x)))
-    return y, z
+    return y, slope
 
 
 class _CompressedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, bias, residual, w, act, width):
         with _lib.on_device_of(x):
-            y, z = _forward(x, w, bias, act, width, residual, act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]))
-        ctx.save_for_backward(z, w.codes, w.scale, w.zero_point)
+            y, slope = _forward(x, w, bias, act, width, residual, act != 0 and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]))
+        ctx.save_for_backward(slope, w.codes, w.scale, w.zero_point)
         ctx.weight, ctx.act, ctx.shape, ctx.dtype = w[3:], act, x.shape, x.dtype
         return y.reshape(x.shape[:-1] + (width,))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        z, codes, scale, zp = ctx.saved_tensors
+        slope, codes, scale, zp = ctx.saved_tensors
         w = PackedWeight(codes, scale, zp, *ctx.weight)
         need_x, need_bias, need_residual = ctx.needs_input_grad[:3]
         dx = dbias = None
         if need_x or need_bias:
             with _lib.on_device_of(dy):
-                dz, ldz, dbias = activation_grad(dy, z, w.n, ctx.act, ctx.dtype, need_x, need_bias)
+                dz, ldz, dbias = activation_grad(dy, slope, w.n, ctx.act, ctx.dtype, need_x, need_bias)
                 if need_x:
                     dx = grad_input(dz, ldz, w, None, ctx.dtype).reshape(ctx.shape)
         return dx, dbias, dy if need_residual else None, None, None, None
@@ -215,8 +215,8 @@ def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias:
                  silu(gate) * up has out_features / 2 columns
     residual     the result's shape and type
 
-    Differentiable in x, bias and residual (not twice); the weight is frozen.  With an activation the backward pass keeps the
-    sums in x's type."""
+    Differentiable in x, bias and residual (not twice); the weight is frozen.  With an activation the backward pass keeps its
+    slope at every sum, in fp32."""
     what = "compressed_linear"
     _lib.require_gpu(x, what)
     w = packed_weight(packed, decompressor, x, 2, what)

@@ -75,7 +75,7 @@ def test_strided_and_misaligned_rows(m):
 
 @pytest.mark.parametrize("m", [97, 257])
 def test_train_where_the_forward_pass_runs_on_the_codes(m):
-    """z is kept by the kernel that joins the parts of k (or by the tiles' own): the gradients see it."""
+    """The slopes are kept by the kernel that joins the parts of k (or by the tiles' own): the gradients see them."""
     from nncf_amd.linear import compressed_linear
     dtype, n, k = torch.bfloat16, 520, 2048
     for mode, act in (("int4_asym", "gelu"), ("nf4", "swiglu"), ("int8_sym", "silu")):
@@ -143,3 +143,36 @@ def test_offsets_beyond_31_bits():
         assert_within(y[:, :512], want, by)
         want, by = plain(x, w[-512:])
         assert_within(y[:, -512:], want, by)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "silu", "swiglu"])
+@pytest.mark.parametrize("m", [1, 60, 333])
+def test_bias_gradient_is_rounded_once(m, act, dtype):
+    """Between dy and dbias nothing is rounded to 16 bits: the slopes are those of the fp32 sums and are kept as they are.  With
+    u = 2^-24: a sum z of K products is off by ez <= 2 (K + 2) u sum|x w| (and the bias), a slope by at most 1.2 ez and by 32 u
+    (1 + |z|) of its arithmetic (swiglu: that of silu times the other half, which is off by its own ez), and m of them times dy
+    are added up in fp32: 2 (m + 2) u of their magnitudes.  Then dbias is rounded, half a step."""
+    from nncf_amd.linear import compressed_linear
+    from tests.linear_utils import act64
+    n, k, u, half = 320, 256, 2.0 ** -24, torch.finfo(dtype).eps / 2
+    packed, dec = make_weight("int4_sym", 64, (n, k), dtype, seed=m)
+    x, bias = _rows(m, k, dtype, m) * 0.3, _rows(1, n, dtype, m + 1)[0].requires_grad_()
+    y = compressed_linear(x, packed, dec, bias=bias, activation=act)
+    dy = _rows(m, y.shape[-1], dtype, m + 2)
+    y.backward(dy)
+    w, d = dec(packed).double(), dy.double()
+    z = (x.double() @ w.t() + bias.detach().double()).requires_grad_()
+    dz = torch.autograd.grad(act64(z, act), z, d)[0]
+    z = z.detach()
+    ez = 2 * (k + 2) * u * (x.double().abs() @ w.abs().t() + bias.detach().double().abs())
+    if act == "swiglu":
+        (a, b), (ea, eb) = z.chunk(2, -1), ez.chunk(2, -1)
+        off = torch.cat((d.abs() * (1.2 * (ea * b.abs() + eb) + 32 * u * (1 + a.abs()) * b.abs()),
+                         d.abs() * (1.2 * ea + 32 * u * (1 + a.abs()) * (1 + a.abs()))), -1)
+    else:
+        off = d.abs() * (1.2 * ez + 32 * u * (1 + z.abs()))
+    off = off.sum(0) + 2 * (m + 2) * u * (dz.abs() + off).sum(0)
+    want = dz.sum(0)
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    assert_within(bias.grad, want, off + half * (want.abs() + off) + tiny)
