@@ -176,3 +176,33 @@ def test_bias_gradient_is_rounded_once(m, act, dtype):
     want = dz.sum(0)
     tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
     assert_within(bias.grad, want, off + half * (want.abs() + off) + tiny)
+
+
+def test_a_call_leaves_nothing_allocated():
+    """Without the collector of cycles: what a call and its gradients allocate is freed when its results are."""
+    import gc
+    from nncf_amd.experts import combine_experts, expert_linear, route_experts
+    from nncf_amd.linear import compressed_linear
+    dtype = torch.bfloat16
+    one, many = make_weight("int4_sym", 64, (256, 512), dtype), make_weight("nf4", 32, (4, 256, 512), dtype)
+
+    def step(m):
+        x, bias = _rows(m, 512, dtype, m).requires_grad_(), torch.zeros(256, dtype=dtype, device="cuda", requires_grad=True)
+        compressed_linear(x, *one, bias=bias, activation="gelu").sum().backward()
+        logits = torch.randn(m, 4, device="cuda", requires_grad=True)
+        r = route_experts(logits, 2)
+        combine_experts(expert_linear(x, *many, r, activation="swiglu"), r).float().sum().backward()
+
+    for m in (1, 100):
+        step(m)
+    gc.collect()
+    gc.disable()
+    try:
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        for m in (1, 100, 1, 100):
+            step(m)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
