@@ -206,3 +206,75 @@ def test_a_call_leaves_nothing_allocated():
         assert torch.cuda.memory_allocated() == before
     finally:
         gc.enable()
+
+
+@pytest.mark.parametrize("m", [4, 90, 300])
+def test_a_captured_training_step_follows_its_inputs(m):
+    """Forward and gradients in one graph: five replays with other inputs, eager work of the same operators between them, and a
+    second graph of the same step captured beside the first."""
+    from nncf_amd.experts import combine_experts, expert_linear, route_experts
+    from nncf_amd.linear import compressed_linear
+    dtype = torch.bfloat16
+    one, many = make_weight("int4_asym", 64, (512, 512), dtype, seed=1), make_weight("mxfp4", 32, (4, 256, 512), dtype, seed=2)
+
+    def step(x, bias, logits, dy):
+        h = compressed_linear(x, *one, bias=bias, activation="gelu")
+        r = route_experts(logits, 2)
+        y = combine_experts(expert_linear(h, *many, r, activation="swiglu"), r)
+        return (y,) + torch.autograd.grad(y, (x, bias, logits), dy)
+
+    def inputs(seed):
+        return [(_rows(m, 512, dtype, seed) * 0.1).requires_grad_(), _rows(1, 512, dtype, seed + 1)[0].requires_grad_(),
+                _rows(m, 4, torch.float32, seed + 2).requires_grad_(), _rows(m, 128, dtype, seed + 3)]
+
+    cases = [inputs(10 * s) for s in range(4)]
+    want = [step(*c) for c in cases]
+    for t in want[0]:
+        assert bool(torch.isfinite(t).all())
+    want = [[t.detach().clone() for t in w] for w in want]
+    graphs = []
+    for _ in range(2):
+        static = [t.detach().clone().requires_grad_(t.requires_grad) for t in cases[0]]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((graph, static, out))
+    for i in (1, 3, 0, 2, 2):
+        for graph, static, out in graphs:
+            with torch.no_grad():
+                for t, c in zip(static, cases[i]):
+                    t.copy_(c)
+            graph.replay()
+        step(*cases[(i + 1) % 4])  # eager work between the replays
+        torch.cuda.synchronize()
+        for graph, static, out in graphs:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
+
+
+def test_two_graphs_replayed_at_once():
+    """Each capture has its own workspace: replays on two streams at the same time give what each gives alone."""
+    from nncf_amd.linear import compressed_linear
+    packed, dec = make_weight("nf4", 64, (1024, 4096), torch.bfloat16, seed=4)
+    xs = [_rows(m, 4096, torch.bfloat16, m) for m in (97, 200, 12)]
+    want = [compressed_linear(x, packed, dec) for x in xs]
+    graphs, outs = [], []
+    for x in xs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(compressed_linear(x, packed, dec))
+        graphs.append((graph, torch.cuda.Stream()))
+    for _ in range(5):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
