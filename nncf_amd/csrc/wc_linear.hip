@@ -423,7 +423,8 @@ Need forward_need(const Weight& w, const void* x, int64_t ldx, int64_t sources, 
         d.few = (double)d.shape.cost * 0.12 < us;
         if (d.few) us = (double)d.shape.cost * 0.12;
     }
-    if (rows <= 4096 * w.experts && w.k == padded(w.k) && codes_fits(w.mode, w.n, w.k, w.gs, w.codes)) {
+    // (tiles are not asked where strips win by far: a search of a microsecond in calls of ten)
+    if ((!d.few || rows > 32 * w.experts) && rows <= 4096 * w.experts && w.k == padded(w.k) && codes_fits(w.mode, w.n, w.k, w.gs, w.codes)) {
         d.codes = codes_plan(w.mode, w.n, w.k, gated, rows, w.experts, grouped);
         d.tiles = d.codes.us < us;
         if (d.tiles) d.few = false;

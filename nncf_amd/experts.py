@@ -17,7 +17,7 @@ from nncf_amd import _lib
 from nncf_amd import decompressors as dcmp
 from nncf_amd.errors import InternalError
 from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_of, grad_input, packed_weight, ptr, rows_of,
-                             workspace_of)
+                             workspace_bytes, workspace_of)
 from nncf_amd.parameters import CompressWeightsMode, as_config
 
 MAX_EXPERTS, MAX_TOPK = 1024, 64
@@ -48,7 +48,7 @@ def _route(logits, top_k, renormalize, mask):
     ints = torch.empty(3 * slots + experts + 1, dtype=torch.int32, device=logits.device)
     at = ints.data_ptr()
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_route_experts_workspace(tokens, experts, top_k), logits.device)
+    ws = workspace_of(workspace_bytes("nncf_amd_route_experts_workspace", tokens, experts, top_k), logits.device)
     _lib.check(L.nncf_amd_route_experts(rows.data_ptr(), _lib.dtype_id(rows), ldl, tokens, experts, top_k, int(renormalize), ptr(mask),
                                         weights.data_ptr(), at, at + 4 * slots, at + 8 * slots, at + 12 * slots, ptr(ws),
                                         0 if ws is None else ws.numel(), _lib.raw_stream(logits)))
@@ -140,8 +140,8 @@ def _expert_forward(x, w: PackedWeight, slots, offsets, rows: int, top_k: int, g
     y = torch.empty((rows, width), dtype=x.dtype, device=x.device)
     slope = torch.empty((rows, w.n), dtype=torch.float32, device=x.device) if want_slope else None
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_expert_linear_workspace(ptr(src), ldx, src.shape[0], int(gather), rows, w.n, w.k, ptr(w.codes), w.mode,
-                                                         w.group_size, w.experts, act), x.device)
+    ws = workspace_of(workspace_bytes("nncf_amd_expert_linear_workspace", src.data_ptr() & 15, ldx, src.shape[0], int(gather), rows,
+                                      w.n, w.k, w.codes.data_ptr() & 15, w.mode, w.group_size, w.experts, act), x.device)
     _lib.check(L.nncf_amd_expert_linear(ptr(src), _DTYPES[x.dtype], ldx, src.shape[0], ptr(slots) if gather else None, top_k,
                                         ptr(offsets), w.experts, rows, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
                                         ptr(w.scale), ptr(w.zero_point), act, ptr(y), width, ptr(slope), ptr(ws),

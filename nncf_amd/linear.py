@@ -10,6 +10,7 @@ sums are fp32 and the result is rounded once.
 """
 from __future__ import annotations
 
+import functools
 import math
 import types
 from typing import NamedTuple, Optional, Tuple
@@ -129,6 +130,12 @@ def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=8192)
+def workspace_bytes(query: str, *numbers: int) -> int:
+    """What a size query of the library answers: it depends on its numbers alone (on addresses by their alignment to 16 bytes)."""
+    return getattr(_lib.lib(), query)(*numbers)
+
+
 def workspace_of(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -145,7 +152,7 @@ def activation_grad(dy: torch.Tensor, slope: Optional[torch.Tensor], n: int, act
     ldz = (n + 63) // 64 * 64
     dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
     dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
-    ws = workspace_of(L.nncf_amd_activation_grad_workspace(m, n) if want_dbias else 0, dy.device)
+    ws = workspace_of(workspace_bytes("nncf_amd_activation_grad_workspace", m, n) if want_dbias else 0, dy.device)
     _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(slope), m, n, act, ptr(dz), ldz, ptr(dbias),
                                           ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dy)))
     return (dz, ldz, dbias) if copies else (dy, ldd, dbias)
@@ -156,7 +163,7 @@ def grad_input(dz: torch.Tensor, ldz: int, w: PackedWeight, offsets: Optional[to
     L = _lib.lib()
     m = dz.shape[0]
     dx = torch.empty((m, w.k), dtype=torch.float32 if fp32 else dtype, device=dz.device)
-    ws = workspace_of(L.nncf_amd_linear_grad_input_workspace(ptr(dz), ldz, m, w.n, w.k, w.experts), dz.device)
+    ws = workspace_of(workspace_bytes("nncf_amd_linear_grad_input_workspace", dz.data_ptr() & 15, ldz, m, w.n, w.k, w.experts), dz.device)
     _lib.check(L.nncf_amd_linear_grad_input(ptr(dz), _DTYPES[dtype], ldz, ptr(offsets), w.experts, m, w.n, w.k, ptr(w.codes),
                                             w.mode, w.group_size, ptr(w.scale), ptr(w.zero_point), ptr(dx), w.k, int(fp32),
                                             ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dz)))
@@ -171,8 +178,8 @@ def _forward(x, w: PackedWeight, bias, act: int, width: int, residual, want_slop
     slope = torch.empty((m, w.n), dtype=torch.float32, device=x.device) if want_slope else None
     res, ldr = (None, 0) if residual is None else rows_of(residual, width)
     L = _lib.lib()
-    ws = workspace_of(L.nncf_amd_compressed_linear_workspace(ptr(rows), ldx, m, w.n, w.k, ptr(w.codes), w.mode,
-                                                             w.group_size, act), x.device)
+    ws = workspace_of(workspace_bytes("nncf_amd_compressed_linear_workspace", rows.data_ptr() & 15, ldx, m, w.n, w.k,
+                                      w.codes.data_ptr() & 15, w.mode, w.group_size, act), x.device)
     _lib.check(L.nncf_amd_compressed_linear(ptr(rows), _DTYPES[x.dtype], ldx, m, w.n, w.k, ptr(w.codes), w.mode, w.group_size,
                                             ptr(w.scale), ptr(w.zero_point), ptr(bias), act, ptr(res), ldr,
                                             ptr(y), width, ptr(slope), ptr(ws), 0 if ws is None else ws.numel(),
