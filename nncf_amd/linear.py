@@ -248,6 +248,9 @@ def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias:
 
 
 # ------------------------------------------------------------------------------------------------------------- models
+_LINEAR_FORWARD = nn.Linear.forward
+
+
 def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:
     plist = self.parametrizations.weight
     if not x.is_cuda or torch.is_autocast_enabled("cuda") or x.dtype != weight_dtype_of(plist[0]):
@@ -255,14 +258,23 @@ def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:
     return compressed_linear(x, plist.original, plist[0], bias=self.bias)
 
 
+def _answers_as_linear(mod: nn.Module) -> bool:
+    """Whether `mod` answers by nn.Linear's own forward (or by the one it was given here): not a subclass that overrides it
+    (adapters) nor a module whose forward was replaced (offloading, wrappers), which would lose what they add."""
+    if not isinstance(mod, nn.Linear) or type(mod).forward is not _LINEAR_FORWARD:
+        return False
+    own = mod.__dict__.get("forward")
+    return own is None or getattr(own, "__func__", None) is _fused_forward
+
+
 def fuse_compressed_linears(model: nn.Module) -> int:
     """Lets every `nn.Linear` of a compressed model (`nncf_amd.compress_weights`, `load_compressed`) whose weight is float16 or
     bfloat16 answer through `compressed_linear` instead of decompressing its weight and calling a library product.  In place;
-    parameters, state_dict keys and `save_compressed` stay as they are, results differ by the sums' order only.  Returns how
-    many modules now do."""
+    parameters, state_dict keys and `save_compressed` stay as they are, results differ by the sums' order only.  A subclass
+    with a forward of its own, or a module whose forward was replaced, stays as it is.  Returns how many modules now do."""
     count = 0
     for mod in model.modules():
-        if not isinstance(mod, nn.Linear) or not parametrize.is_parametrized(mod, "weight"):
+        if not _answers_as_linear(mod) or not parametrize.is_parametrized(mod, "weight"):
             continue
         plist = mod.parametrizations.weight
         if len(plist) != 1 or not isinstance(plist[0], dcmp.BaseWeightsDecompressor) or weight_dtype_of(plist[0]) not in _DTYPES:

@@ -1,0 +1,78 @@
+"""CPU: which modules of a compressed model `fuse_compressed_linears` takes over, and when their forward hands a call back.  The
+decompressor here decompresses on the CPU; `compressed_linear` is not reached (its arguments are on no GPU)."""
+import copy
+
+import pytest
+import torch
+from torch import nn
+from torch.nn.utils import parametrize
+
+from nncf_amd import decompressors as dcmp
+
+
+class _OnCpu(dcmp.INT8SymmetricWeightsDecompressor):
+    def forward(self, x):
+        return (x.to(torch.float16) * self._scale).to(self.result_dtype)
+
+
+def _compressed(mod, seed=0):
+    """`mod`, an nn.Linear, with its weight as int8 codes behind a decompressor."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randint(-128, 128, mod.weight.shape, dtype=torch.int8, generator=g)
+    mod.weight = nn.Parameter(codes, requires_grad=False)
+    dec = _OnCpu(torch.rand(codes.shape[0], 1, generator=g) * 0.01 + 0.001, result_dtype=torch.bfloat16)
+    parametrize.register_parametrization(mod, "weight", dec, unsafe=True)
+    return mod.requires_grad_(False)
+
+
+def _linear(cls=nn.Linear, **kw):
+    torch.manual_seed(0)
+    return _compressed(cls(16, 8, dtype=torch.bfloat16, **kw))
+
+
+class _Scaled(nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _Renamed(nn.Linear):
+    pass
+
+
+def _x(rows=5):
+    return torch.randn(rows, 16, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+
+
+def test_a_subclass_with_its_own_forward_keeps_it():
+    from nncf_amd.linear import fuse_compressed_linears
+    model = nn.Sequential(_linear(_Scaled))
+    want = model(_x())
+    assert fuse_compressed_linears(model) == 0
+    assert torch.equal(model(_x()), want)
+
+
+def test_a_replaced_instance_forward_is_kept():
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear()
+    before = mod.forward
+    mod.forward = lambda x: before(x) + 1000
+    want = mod(_x())
+    assert fuse_compressed_linears(mod) == 0
+    assert torch.equal(mod(_x()), want)
+
+
+def test_linears_that_answer_as_linears_are_fused():
+    from nncf_amd.linear import fuse_compressed_linears
+    model = nn.Sequential(_linear(), _linear(_Renamed), _linear(_Scaled), nn.Linear(8, 8))
+    assert fuse_compressed_linears(model) == 2
+    assert fuse_compressed_linears(model) == 2  # once more: the same two
+    assert fuse_compressed_linears(copy.deepcopy(model)) == 2
+
+
+@pytest.mark.parametrize("cls", [nn.Linear, _Renamed])
+def test_a_call_that_is_handed_back_gives_what_it_gave(cls):
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear(cls)
+    want = mod(_x())
+    assert fuse_compressed_linears(mod) == 1
+    assert torch.equal(mod(_x()), want)  # (on the CPU: the library product)
