@@ -76,3 +76,55 @@ def test_a_call_that_is_handed_back_gives_what_it_gave(cls):
     want = mod(_x())
     assert fuse_compressed_linears(mod) == 1
     assert torch.equal(mod(_x()), want)  # (on the CPU: the library product)
+
+
+class _AsOnGpu(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
+
+class _Adapter(nn.Module):
+    def forward(self, w):
+        return w + 0.25
+
+
+@pytest.fixture
+def reached(monkeypatch):
+    """Calls that reach `compressed_linear` are counted and answered by the plain product of the codes' decompressor alone."""
+    from nncf_amd import linear
+    calls = []
+
+    def plain(x, packed, decompressor, bias=None, activation=None, residual=None):
+        calls.append(1)
+        return nn.functional.linear(x.as_subclass(torch.Tensor), decompressor(packed), bias)
+    monkeypatch.setattr(linear, "compressed_linear", plain)
+    return calls
+
+
+def test_a_fused_linear_calls_the_product(reached):
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear()
+    want = mod(_x())
+    fuse_compressed_linears(mod)
+    assert torch.equal(mod(_x().as_subclass(_AsOnGpu)), want) and len(reached) == 1
+
+
+def test_a_parametrization_added_to_a_fused_weight_counts(reached):
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear()
+    fuse_compressed_linears(mod)
+    parametrize.register_parametrization(mod, "weight", _Adapter())
+    x = _x()
+    want = nn.functional.linear(x, mod.weight, mod.bias)
+    assert torch.equal(mod(x.as_subclass(_AsOnGpu)).as_subclass(torch.Tensor), want) and not reached
+
+
+def test_a_fused_linear_survives_the_loss_of_its_parametrization(reached):
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear()
+    want = mod(_x())
+    weight = mod.weight.detach().clone()
+    fuse_compressed_linears(mod)
+    mod._modules.pop("parametrizations")
+    mod.__class__ = nn.Linear
+    mod.weight = nn.Parameter(weight, requires_grad=False)
+    assert torch.equal(mod(_x()), want) and not reached
