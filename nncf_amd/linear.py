@@ -59,7 +59,8 @@ def weight_dtype_of(decompressor) -> torch.dtype:
     """Type of the weight that `decompressor` returns."""
     if decompressor.result_dtype is not None:
         return decompressor.result_dtype
-    return torch.float16
+    scale = decompressor._buffers["_scale"]
+    return scale.dtype if scale.is_floating_point() else torch.float16
 
 
 def packed_weight(packed: torch.Tensor, decompressor, x: torch.Tensor, ndim: int, what: str) -> PackedWeight:
@@ -251,10 +252,13 @@ _LINEAR_FORWARD = nn.Linear.forward
 
 
 def _only_decompressed(mod: nn.Module):
-    """The parametrizations of `mod`'s weight if a decompressor is all they are (an adapter may have joined it, or left), else None."""
+    """The parametrizations of `mod`'s weight if a decompressor is all they are (an adapter may have joined it, or left) and its
+    scales are as it was made with them (`model.float()` casts them), else None."""
     parametrizations = mod._modules.get("parametrizations")
     plist = None if parametrizations is None else parametrizations._modules.get("weight")
-    return plist if plist is not None and len(plist) == 1 and isinstance(plist[0], dcmp.BaseWeightsDecompressor) else None
+    if plist is None or len(plist) != 1 or not isinstance(plist[0], dcmp.BaseWeightsDecompressor):
+        return None
+    return plist if plist[0]._buffers["_scale"].dtype in (torch.float16, torch.uint8) else None
 
 
 def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -128,3 +128,15 @@ def test_a_fused_linear_survives_the_loss_of_its_parametrization(reached):
     mod.__class__ = nn.Linear
     mod.weight = nn.Parameter(weight, requires_grad=False)
     assert torch.equal(mod(_x()), want) and not reached
+
+
+def test_scales_that_were_cast_keep_the_library_product(reached):
+    """`model.float()` casts the decompressor's scales, whose products the kernels do not make."""
+    from nncf_amd.linear import fuse_compressed_linears, weight_dtype_of
+    mod = _linear(bias=False)
+    fuse_compressed_linears(mod)
+    mod.float()
+    want = mod(_x())
+    assert torch.equal(mod(_x().as_subclass(_AsOnGpu)).as_subclass(torch.Tensor), want) and not reached
+    plain = dcmp.INT8SymmetricWeightsDecompressor(torch.ones(8, 1))
+    assert weight_dtype_of(plain) == torch.float16 and weight_dtype_of(plain.float()) == torch.float32
