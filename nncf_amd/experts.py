@@ -16,8 +16,8 @@ from torch.autograd.function import once_differentiable
 from nncf_amd import _lib
 from nncf_amd import decompressors as dcmp
 from nncf_amd.errors import InternalError
-from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_of, grad_input, packed_weight, ptr, rows_of,
-                             workspace_bytes, workspace_of)
+from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_of, grad_input, packed_weight, ptr, refuse_transforms,
+                             rows_of, workspace_bytes, workspace_of)
 from nncf_amd.parameters import CompressWeightsMode, as_config
 
 MAX_EXPERTS, MAX_TOPK = 1024, 64
@@ -78,6 +78,7 @@ class _Route(torch.autograd.Function):
     def backward(ctx, dweights, _):
         if dweights is None:
             return None, None, None, None
+        refuse_transforms("route_experts", dweights)
         logits, weights, ints = ctx.saved_tensors
         tokens, experts = logits.shape
         rows, ldl = rows_of(logits, experts)
@@ -101,6 +102,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True, to
     and differentiable in `logits`."""
     what = "route_experts"
     _lib.require_gpu(logits, what)
+    refuse_transforms(what, logits)
     if logits.ndim != 2 or logits.shape[1] < 1:
         raise InternalError(f"{what}: logits [tokens, experts] expected, got shape {tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.float16, torch.bfloat16):
@@ -117,7 +119,7 @@ def route_experts(logits: torch.Tensor, top_k: int, renormalize: bool = True, to
         return _routing(*_route(logits, top_k, renormalize, token_mask))
 
 
-def _check_routing(routing: ExpertRouting, device, what: str, experts: Optional[int] = None):
+def _check_routing(routing: ExpertRouting, x: torch.Tensor, what: str, experts: Optional[int] = None):
     """(tokens, top_k) of a routing whose tensors are as `route_experts` makes them."""
     if not isinstance(routing, ExpertRouting):
         raise InternalError(f"{what}: expected the ExpertRouting of route_experts, got {type(routing).__name__}")
@@ -127,9 +129,9 @@ def _check_routing(routing: ExpertRouting, device, what: str, experts: Optional[
             or rows.dtype != torch.int32 or slots.dtype != torch.int32 or offsets.dtype != torch.int32
             or not (weights.is_contiguous() and rows.is_contiguous() and slots.is_contiguous() and offsets.is_contiguous())):
         raise InternalError(f"{what}: the routing's tensors are not as route_experts makes them")
-    index = device.index
+    index = x.get_device()
     if rows.get_device() != index or weights.get_device() != index or slots.get_device() != index or offsets.get_device() != index:
-        raise InternalError(f"{what}: the routing is on {rows.device}, the activations on {device}")
+        raise InternalError(f"{what}: the routing is on {rows.device}, the activations on {x.device}")
     if experts is not None and routing.offsets.numel() != experts + 1:
         raise InternalError(f"{what}: a routing over {routing.offsets.numel() - 1} experts for a stack of {experts}")
     return tokens, top_k
@@ -161,6 +163,7 @@ class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_transforms("expert_linear", dy)
         slope, codes, scale, zp, offsets, places = ctx.saved_tensors
         w = PackedWeight(codes, scale, zp, *ctx.weight)
         with _lib.on_device_of(dy):
@@ -183,9 +186,10 @@ def expert_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, routing: 
     Activations, types and gradients as in `nncf_amd.linear.compressed_linear`; differentiable in x."""
     what = "expert_linear"
     _lib.require_gpu(x, what)
+    refuse_transforms(what, x)
     w = packed_weight(packed, decompressor, x, 3, what)
     act, width = activation_of(activation, w.n, what)
-    tokens, top_k = _check_routing(routing, x.device, what, w.experts)
+    tokens, top_k = _check_routing(routing, x, what, w.experts)
     rows = tokens * top_k
     if x.ndim != 2 or tuple(x.shape) != (tokens if gather else rows, w.k):
         raise InternalError(f"{what}: x of shape {tuple(x.shape)}, expected {(tokens if gather else rows, w.k)}")
@@ -216,6 +220,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        refuse_transforms("combine_experts", dout)
         y, weights, places, slots = ctx.saved_tensors
         tokens, top_k = places.shape
         n = y.shape[1]
@@ -236,7 +241,8 @@ def combine_experts(y: torch.Tensor, routing: ExpertRouting) -> torch.Tensor:
     rounded once; a masked token's is zero.  Differentiable in y and routing.weights."""
     what = "combine_experts"
     _lib.require_gpu(y, what)
-    tokens, top_k = _check_routing(routing, y.device, what)
+    tokens, top_k = _check_routing(routing, y, what)
+    refuse_transforms(what, y, routing.weights)
     if y.dtype not in _DTYPES:
         raise InternalError(f"{what}: rows are float16 or bfloat16, got {y.dtype}")
     if y.ndim != 2 or y.shape[0] != tokens * top_k or y.shape[1] < 1:

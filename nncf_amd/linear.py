@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from nncf_amd import _lib
@@ -61,6 +62,22 @@ def weight_dtype_of(decompressor) -> torch.dtype:
         return decompressor.result_dtype
     scale = decompressor._buffers["_scale"]
     return scale.dtype if scale.is_floating_point() else torch.float16
+
+
+_transforms_active = torch._C._are_functorch_transforms_active
+
+
+def transformed(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of `tensors` carries a forward-mode tangent or comes from a function transform (torch.func)."""
+    if forward_ad._current_level < 0 and not _transforms_active():
+        return False
+    return any(t is not None and (torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None)
+               for t in tensors)
+
+
+def refuse_transforms(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if transformed(*tensors):
+        raise InternalError(f"{what}: forward-mode derivatives and function transforms are not supported")
 
 
 def packed_weight(packed: torch.Tensor, decompressor, x: torch.Tensor, ndim: int, what: str) -> PackedWeight:
@@ -199,6 +216,7 @@ class _CompressedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_transforms("compressed_linear", dy)
         slope, codes, scale, zp = ctx.saved_tensors
         w = PackedWeight(codes, scale, zp, *ctx.weight)
         need_x, need_bias, need_residual = ctx.needs_input_grad[:3]
@@ -222,10 +240,11 @@ def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias:
                  silu(gate) * up has out_features / 2 columns
     residual     the result's shape and type
 
-    Differentiable in x, bias and residual (not twice); the weight is frozen.  With an activation the backward pass keeps its
+    Differentiable in x, bias and residual (in reverse mode, not twice); the weight is frozen.  With an activation the backward pass keeps its
     slope at every sum, in fp32."""
     what = "compressed_linear"
     _lib.require_gpu(x, what)
+    refuse_transforms(what, x, bias, residual)
     w = packed_weight(packed, decompressor, x, 2, what)
     act, width = activation_of(activation, w.n, what)
     if x.ndim < 1 or x.shape[-1] != w.k:
@@ -265,7 +284,10 @@ def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:
     plist = _only_decompressed(self)
     if plist is None or not x.is_cuda or torch.is_autocast_enabled("cuda") or x.dtype != weight_dtype_of(plist[0]):
         return nn.Linear.forward(self, x)  # a library product of the weight as it is now, as before
-    return compressed_linear(x, plist.original, plist[0], bias=self.bias)
+    bias = self.bias
+    if transformed(x, bias):
+        return nn.Linear.forward(self, x)
+    return compressed_linear(x, plist.original, plist[0], bias=bias)
 
 
 def _answers_as_linear(mod: nn.Module) -> bool:
@@ -280,8 +302,10 @@ def _answers_as_linear(mod: nn.Module) -> bool:
 def fuse_compressed_linears(model: nn.Module) -> int:
     """Lets every `nn.Linear` of a compressed model (`nncf_amd.compress_weights`, `load_compressed`) whose weight is float16 or
     bfloat16 answer through `compressed_linear` instead of decompressing its weight and calling a library product.  In place;
-    parameters, state_dict keys and `save_compressed` stay as they are, results differ by the sums' order only.  A subclass
-    with a forward of its own, or a module whose forward was replaced, stays as it is.  Returns how many modules now do."""
+    parameters, state_dict keys and `save_compressed` stay as they are, results differ by the sums' order only; their
+    gradients can be taken once.  A subclass with a forward of its own, or a module whose forward was replaced, stays as it is;
+    calls on the CPU, under autocast, in another type, in forward mode or under a function transform go the former way.  Returns
+    how many modules now answer so."""
     count = 0
     for mod in model.modules():
         plist = _only_decompressed(mod) if _answers_as_linear(mod) else None
