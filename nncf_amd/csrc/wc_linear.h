@@ -344,7 +344,7 @@ struct FewShape {
     int lds_rows, tiles;          // and that LDS holds; tiles of 16 of them
     int steps, per_wk;            // steps of a wave; ceil(2^16 / wk)
     int kz;                       // blocks that share k: above 1 they leave fp32 sums [kz][rows][n] in the workspace
-    int pitch;                    // groups of a row, and one place more
+    int pitch;                    // groups of a row, and a place behind them (groups of 32: two, a quarter reads both)
     int scale_bytes, zero_bytes;  // per group; zero_bytes 0: none
     int x_bytes;                  // of a row and step
     int64_t cost;                 // its time in units of 0.12 us

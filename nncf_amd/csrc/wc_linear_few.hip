@@ -201,11 +201,13 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
                     }
                 }
             }
-            // an odd number of groups of 32 ends in half a quarter; the other half meets x's zeros
-            for (int r = threadIdx.x; r < sh.wn * 16; r += blockDim.x) {
-                put_scale(((r >> 4) * sh.pitch + a.groups) * 16 + (r & 15), 0);
-                if constexpr (ASYM) zeros[((r >> 4) * sh.pitch + a.groups) * 16 + (r & 15)] = 0;
-            }
+            // What lies behind the last group, half a quarter of an odd number of groups of 32 among it, has scale 0: whatever
+            // codes stand there, their values are finite and meet x's zeros (under another group's scale they could be infinite).
+            for (uint32_t g = a.groups; g < (uint32_t)sh.pitch; ++g)
+                for (int r = threadIdx.x; r < sh.wn * 16; r += blockDim.x) {
+                    put_scale(((r >> 4) * sh.pitch + g) * 16 + (r & 15), 0);
+                    if constexpr (ASYM) zeros[((r >> 4) * sh.pitch + g) * 16 + (r & 15)] = 0;
+                }
         }
         fresh = false;
         put_x(0);
@@ -237,7 +239,7 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const uint32_t kk = stage_of(s) * KS + q * (KS / 4), at = __umulhi(kk / 16, a.magic);
-                const int gi = group0 + 16 * (int)(at < a.groups ? at : a.groups - 1);  // (behind the end of k: any)
+                const int gi = group0 + 16 * (int)(at < a.groups ? at : a.groups);  // (behind the end of k: scale 0)
                 const GroupPar<MODE> g = par_of<MODE>(scales[gi], ASYM ? zeros[gi] : 0);
                 const u32v2 c = *(const u32v2*)(mine + get + (((2 * q + (kq >> 1)) ^ (r16 >> 1)) << 4));
                 if constexpr (MF == 2) {
@@ -344,7 +346,7 @@ FewShape few_shape(int mode, int64_t k, int64_t groups, int wn, int wk, int kz, 
     const bool four = four_bit(mode);
     const int64_t stages = (k + (four ? 255 : 127)) / (four ? 256 : 128);
     const int steps = (int)((stages + (int64_t)wk * kz - 1) / ((int64_t)wk * kz));
-    return FewShape{wn, wk, rows, steps > 1 ? 2 : 1, tiles > 1 ? 16 * tiles : rows, tiles, steps, (65536 + wk - 1) / wk, kz, (int)groups + 1,
+    return FewShape{wn, wk, rows, steps > 1 ? 2 : 1, tiles > 1 ? 16 * tiles : rows, tiles, steps, (65536 + wk - 1) / wk, kz, (int)groups + (groups * 32 == k ? 2 : 1),
                     mode == NNCF_AMD_MXFP4 ? 1 : 2, mode == NNCF_AMD_INT4_ASYM || mode == NNCF_AMD_INT8_ASYM ? 1 : 0, four ? 512 : 256, 0};
 }
 
