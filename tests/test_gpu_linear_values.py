@@ -46,3 +46,67 @@ def test_a_large_scale_meets_its_own_codes_only(mode, gs, n, k, dtype, m):
     x = _rows(m, k, dtype, m) * (2.0 ** -10)
     y, by = plain(x, w)
     assert_within(compressed_linear(x, packed, dec), y, by)
+
+
+def _identity(k, dtype):
+    """A weight of ones on the diagonal: the sums are x itself."""
+    from nncf_amd import decompressors as D
+    return torch.eye(k, dtype=torch.int8, device="cuda"), D.INT8SymmetricWeightsDecompressor(torch.ones(k, 1, device="cuda"), result_dtype=dtype)
+
+
+def _every_value(dtype, k, reach):
+    """All numbers of a 16-bit type up to `reach` on both sides as rows of k (the last one filled up with zeros)."""
+    v = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    v = v[torch.isfinite(v) & (v.abs() <= reach)]
+    return torch.cat((v, v.new_zeros(-v.numel() % k))).view(-1, k).cuda()
+
+
+def _in_pieces(x, m, call):
+    return torch.cat([call(x[r:r + m]) for r in range(0, x.shape[0], m)])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("m", [1, 100, 1024])
+def test_activations_are_right_to_their_last_place(m, act, dtype):
+    """Every value of x: an activation is off by a share of ITSELF, also far out on the left, where it is small.  With u = 2^-24:
+    the exponential of an argument a, rounded twice or three times on its way, is off by 3 u |a| of itself, its instruction, a
+    reciprocal and a handful of products, sums of positive terms and a fitted polynomial (7e-7) by 40 u; then y is rounded once.
+    |a| is z^2 / 2, 2 sqrt(2 / pi) |z + 0.044715 z^3| or |z|.  z's factor may be flushed below the smallest normal number, 2^-126:
+    that takes 2^-126 |z| from the product, and the product itself may be flushed."""
+    from nncf_amd.linear import compressed_linear
+    k, u = 256, 2.0 ** -24
+    packed, dec = _identity(k, dtype)
+    x = _every_value(dtype, k, 80.0 if act == "silu" else 12.5)
+    got = _in_pieces(x, m, lambda t: compressed_linear(t, packed, dec, activation=act))
+    z = x.double()
+    if act == "gelu":
+        want, a = z * 0.5 * torch.erfc(-z * 0.5 ** 0.5), z * z / 2
+    else:
+        a = z if act == "silu" else 1.5957691216057308 * (z + 0.044715 * z ** 3)
+        want = z * torch.sigmoid(a)
+    off = want.abs() * (40 * u + 3 * u * a.abs()) + 2.0 ** -126 * (1 + z.abs())
+    half = torch.finfo(dtype).eps / 2
+    assert_within(got, want, off + (want.abs() + off) * half + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 1024])
+def test_the_slope_of_gelu_is_right_to_its_last_place(m, dtype):
+    """As above for Phi(z) + z phi(z) with dy = 1: each of the two is off by a share of itself, dz is rounded once, dx (one product)
+    once more without another error."""
+    from nncf_amd.linear import compressed_linear
+    k, u = 256, 2.0 ** -24
+    packed, dec = _identity(k, dtype)
+    x = _every_value(dtype, k, 12.5)
+
+    def gradient(t):
+        t = t.clone().requires_grad_(True)
+        return torch.autograd.grad(compressed_linear(t, packed, dec, activation="gelu"), t, torch.ones_like(t))[0]
+    got = _in_pieces(x, m, gradient)
+    z = x.double()
+    cdf, rest = 0.5 * torch.erfc(-z * 0.5 ** 0.5), z * torch.exp(-z * z / 2) * 0.3989422804014327
+    want = cdf + rest
+    off = (cdf + rest.abs()) * (40 * u + 3 * u * z * z / 2) + 2.0 ** -126 * (1 + z.abs())
+    half = torch.finfo(dtype).eps / 2
+    assert_within(got, want, off + (want.abs() + off) * half + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2)
