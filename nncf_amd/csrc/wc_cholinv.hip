@@ -320,13 +320,10 @@ extern "C" int nncf_amd_cholinv_block(const float* a, int64_t lda, float* linv, 
     }
     constexpr size_t lds_bytes = (size_t)(2 * CB * CLD + 2 * CB + 2) * sizeof(float);  // ~130 KiB of dynamic LDS
     static OncePerDevice attr_once;
-    if (attr_once.first_on_device() != 0) {
-        if (hipFuncSetAttribute((const void*)k_cholinv_block, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                (int)lds_bytes) != hipSuccess) {
-            attr_once.forget_current();
-            return launch_status("cholinv_block attribute");
-        }
-    }
+    const bool opted_in = attr_once.run([&] {
+        return hipFuncSetAttribute((const void*)k_cholinv_block, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess;
+    });
+    if (!opted_in) return launch_status("cholinv_block attribute");
     static const bool per_column = [] { const char* e = getenv("NNCF_AMD_CHOLINV_PER_COLUMN"); return e && e[0] == '1'; }();
     if (per_column) {  // (developer knob: the one-barrier-per-column form)
         hipLaunchKernelGGL(k_cholinv_block, dim3(1), dim3(256), lds_bytes, (hipStream_t)stream, a, lda, linv, ldo, (int)n,
@@ -335,13 +332,10 @@ extern "C" int nncf_amd_cholinv_block(const float* a, int64_t lda, float* linv, 
     }
     constexpr size_t lds16 = (size_t)(CB * CLD + 3 + 2 * CB * PP + 4 * PB * PP) * sizeof(float);
     static OncePerDevice attr16;
-    if (attr16.first_on_device() != 0) {
-        if (hipFuncSetAttribute((const void*)k_cholinv_block16, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds16) !=
-            hipSuccess) {
-            attr16.forget_current();
-            return launch_status("cholinv_block16 attribute");
-        }
-    }
+    const bool opted_in16 = attr16.run([&] {
+        return hipFuncSetAttribute((const void*)k_cholinv_block16, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds16) == hipSuccess;
+    });
+    if (!opted_in16) return launch_status("cholinv_block16 attribute");
     hipLaunchKernelGGL(k_cholinv_block16, dim3(1), dim3(256), lds16, (hipStream_t)stream, a, lda, linv, ldo, (int)n, info);
     return launch_status("cholinv_block");
 }

@@ -5,9 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
-
 #include "../../include/nncf_amd_wc.h"
+#include "wc_once.h"
 
 namespace wc {
 
@@ -16,25 +15,13 @@ constexpr float kEps = 1.1920928955078125e-07f;  // 2^-23 == fns.finfo(float32).
 void set_error(const char* fmt, ...);
 int launch_status(const char* what);
 
-// Per-device "done once" flag for attribute opt-ins (hipFuncSetAttribute is per device): first_on_device() is true
-// the first time it is asked on the current device and false afterwards; thread-safe.
-struct OncePerDevice {
-    std::mutex m;
-    bool seen[64] = {};
-    // returns -1: cannot tell the device, 1: first call on it, 0: seen before
-    int first_on_device() {
+// The attribute opt-ins (hipFuncSetAttribute is per device): true once `action` has succeeded on the current device.
+struct OncePerDevice : OncePerKey {
+    template <class Action>
+    bool run(Action&& action) {
         int dev = -1;
-        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -1;
-        std::lock_guard<std::mutex> lock(m);
-        if (seen[dev]) return 0;
-        seen[dev] = true;
-        return 1;
-    }
-    void forget_current() {  // the opt-in failed: try again next time
-        int dev = -1;
-        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return;
-        std::lock_guard<std::mutex> lock(m);
-        seen[dev] = false;
+        if (hipGetDevice(&dev) != hipSuccess) dev = -1;
+        return OncePerKey::run(dev, action);
     }
 };
 

@@ -263,12 +263,10 @@ int codes_tiles(const CodesArgs& a, hipStream_t s) {
     static OncePerDevice once;
     constexpr int kLds = CodesLds<MODE, FB>::total, PB = 32 * WJ * FB;
     static_assert(kLds + (MODE == NNCF_AMD_NF4 ? 4 * kNf4Pairs : 0) <= 160 * 1024, "LDS of a compute unit");
-    const int first = once.first_on_device();
-    if (first < 0 || (first && hipFuncSetAttribute((const void*)k_gemm_codes<MODE, DT, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess)) {
-        if (first > 0) once.forget_current();
-        set_error("linear: LDS refused");
-        return NNCF_AMD_ERR_LAUNCH;
-    }
+    const bool opted_in = once.run([&] {
+        return hipFuncSetAttribute((const void*)k_gemm_codes<MODE, DT, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+    });
+    if (!opted_in) return lds_refused(kLds);
     const bool halves = a.ep.act == kActSwiglu && a.kz == 1;
     const int64_t tiles_n = ((halves ? a.ep.n / 2 : a.ep.n) + (halves ? 63 : 127)) / (halves ? 64 : 128);
     const int64_t groups = a.rows.offsets ? (a.rows.experts < a.rows.rows ? a.rows.experts : a.rows.rows) : 1;

@@ -228,16 +228,10 @@ int dense_tiles(const DenseArgs& a, hipStream_t s) {
     constexpr int PA = 32 * WI * FA, PB = 32 * WJ * FB, kStageLds = kSlots * PA * kRowBytes;
     constexpr int kTileLds = WI * WJ * kTileFloats<FA> * 4;  // the epilogue's floats take the stages' place
     constexpr int kLds = kStageLds > kTileLds ? kStageLds : kTileLds;
-    const int first = once.first_on_device();
-    if (first < 0) {
-        set_error("linear: no current device");
-        return NNCF_AMD_ERR_LAUNCH;
-    }
-    if (first && hipFuncSetAttribute((const void*)k_gemm_nt<DT, WI, WJ, FA, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) != hipSuccess) {
-        once.forget_current();
-        set_error("linear: %d bytes of LDS refused", kLds);
-        return NNCF_AMD_ERR_LAUNCH;
-    }
+    const bool opted_in = once.run([&] {
+        return hipFuncSetAttribute((const void*)k_gemm_nt<DT, WI, WJ, FA, FB>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds) == hipSuccess;
+    });
+    if (!opted_in) return lds_refused(kLds);
     const bool gated = a.ep.act == kActSwiglu;
     const int64_t width = gated ? a.ep.n / 2 : a.ep.n, per = gated ? PA / 2 : PA, pb = PB;
     const int64_t tiles_n = (width + per - 1) / per;

@@ -179,7 +179,7 @@ extern "C" int nncf_amd_gptq_block(const float* weight, float* quantized, float*
                            err_block, hinv, rows, k, i1, (int)count, gs, mode, scales, zps, use_given_params);
     };
     static OncePerDevice attr_once;
-    if (attr_once.first_on_device() != 0) {
+    const bool opted_in = attr_once.run([&] {
         bool ok = true;
         auto opt_in = [&](auto kernel) {
             ok = ok && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)hb_bytes) == hipSuccess;
@@ -187,11 +187,9 @@ extern "C" int nncf_amd_gptq_block(const float* weight, float* quantized, float*
         opt_in(k_gptq_block<IntPolicy, 4>), opt_in(k_gptq_block<IntPolicy, 8>), opt_in(k_gptq_block<IntPolicy, 16>);
         opt_in(k_gptq_block<FloatPolicy<true>, 4>), opt_in(k_gptq_block<FloatPolicy<true>, 8>), opt_in(k_gptq_block<FloatPolicy<true>, 16>);
         opt_in(k_gptq_block<FloatPolicy<false>, 4>), opt_in(k_gptq_block<FloatPolicy<false>, 8>), opt_in(k_gptq_block<FloatPolicy<false>, 16>);
-        if (!ok) {
-            attr_once.forget_current();
-            return launch_status("gptq_block attribute");
-        }
-    }
+        return ok;
+    });
+    if (!opted_in) return launch_status("gptq_block attribute");
     auto by_lanes = [&](auto k4, auto k8, auto k16) {
         if (lanes_per_row == 4) launch(k4, 4);
         else if (lanes_per_row == 8) launch(k8, 8);

@@ -1016,13 +1016,11 @@ static int launch_syrk16b_list(float* h, const wc::SyrkItems& items, int x_dtype
     static const int64_t list_min_tiles = [] { const char* e = getenv("NNCF_AMD_SYRK_LIST_TILES"); return e ? atoll(e) : 48ll; }();  // developer knob
     if (nt >= list_min_tiles) {
         static OncePerDevice attr_list;
-        if (attr_list.first_on_device() != 0) {
-            if (hipFuncSetAttribute((const void*)k_gemm16t_list<NNCF_AMD_BF16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess ||
-                hipFuncSetAttribute((const void*)k_gemm16t_list<NNCF_AMD_F16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess) {
-                attr_list.forget_current();
-                return launch_status("hessian gemm16t_list attribute");
-            }
-        }
+        const bool opted_in = attr_list.run([&] {
+            return hipFuncSetAttribute((const void*)k_gemm16t_list<NNCF_AMD_BF16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess &&
+                   hipFuncSetAttribute((const void*)k_gemm16t_list<NNCF_AMD_F16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess;
+        });
+        if (!opted_in) return launch_status("hessian gemm16t_list attribute");
         Gemm16Args g = {h, nullptr, nullptr, 0u, 0u, (uint32_t)k, (uint32_t)k, (uint32_t)k, (uint32_t)k, (uint32_t)k, nt, nt,
                         (int)stages, (int)sp, 4, 1, (uint32_t)prs, alpha};
         const int64_t blocks = ((prs + 7) / 8) * sp * 8;
@@ -1033,13 +1031,11 @@ static int launch_syrk16b_list(float* h, const wc::SyrkItems& items, int x_dtype
         return launch_status("hessian_gemm16t_list");
     }
     static OncePerDevice attr_once;
-    if (attr_once.first_on_device() != 0) {
-        if (hipFuncSetAttribute((const void*)k_syrk16b<NNCF_AMD_BF16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess ||
-            hipFuncSetAttribute((const void*)k_syrk16b<NNCF_AMD_F16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess) {
-            attr_once.forget_current();
-            return launch_status("hessian_syrk16b attribute");
-        }
-    }
+    const bool opted_in = attr_once.run([&] {
+        return hipFuncSetAttribute((const void*)k_syrk16b<NNCF_AMD_BF16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess &&
+               hipFuncSetAttribute((const void*)k_syrk16b<NNCF_AMD_F16>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess;
+    });
+    if (!opted_in) return launch_status("hessian_syrk16b attribute");
     const dim3 grid((unsigned)prs, (unsigned)sp);
     if (x_dtype == NNCF_AMD_BF16)
         hipLaunchKernelGGL((k_syrk16b<NNCF_AMD_BF16>), grid, dim3(256), lds_bytes, s, h, items, k, alpha, nt, (int)sps);
@@ -1281,12 +1277,10 @@ extern "C" int nncf_amd_gemm_bf16_tn_acc(float* c, int64_t ldc, const void* p, i
     }
     constexpr size_t lds_bytes = (size_t)GST * 2 * GK * GROW;
     static OncePerDevice attr_once;
-    if (attr_once.first_on_device() != 0) {
-        if (hipFuncSetAttribute((const void*)k_gemm16t, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess) {
-            attr_once.forget_current();
-            return launch_status("gemm_bf16_tn_acc attribute");
-        }
-    }
+    const bool opted_in = attr_once.run([&] {
+        return hipFuncSetAttribute((const void*)k_gemm16t, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess;
+    });
+    if (!opted_in) return launch_status("gemm_bf16_tn_acc attribute");
     Gemm16Args g = {c, p, q, (uint32_t)((uint64_t)t * ldp * 2), (uint32_t)((uint64_t)t * ldq * 2), (uint32_t)ldp, (uint32_t)ldq,
                     (uint32_t)ldc, (uint32_t)m, (uint32_t)n, tm, tn, (int)stages, (int)sp, tri, 0, 0, 1.0f};
     // tile order of a triangular product: per-XCD lists where every XCD gets (nearly) the same number of lines

@@ -368,6 +368,7 @@ bool few_fits(int mode, int64_t k, int64_t gs, const void* codes, int64_t source
 // the quickest shape for `rows` rows of x over `experts` weights (grouped: with row offsets)
 FewShape few_plan(int mode, int64_t n, int64_t k, int64_t groups, bool gated, int64_t rows, int64_t experts, bool grouped);
 int few_launch(int dtype, int mode, const FewArgs& a, const FewShape& sh, hipStream_t s);
+int lds_refused(int bytes);  // the error of a launcher whose opt-in to so much LDS failed
 // y from the sums [kz][rows][n] that blocks sharing k left, in the order of their parts
 int join_sums(int dtype, const float* sums, int kz, const RowMap& rows, const Epilogue& ep, hipStream_t s);
 

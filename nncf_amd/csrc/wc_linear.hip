@@ -458,6 +458,12 @@ int pack_rows(const void*& x, int64_t& ldx, int64_t k, RowMap& rows, uint16_t* p
     return launch_status("linear: rows");
 }
 
+int lds_refused(int bytes) {
+    (void)hipGetLastError();  // (reported here, not by the next launch)
+    set_error("linear: %d bytes of LDS refused", bytes);
+    return NNCF_AMD_ERR_LAUNCH;
+}
+
 int out_of_range(int64_t n, int64_t k) {
     set_error("linear: operands beyond the kernels' range (n=%lld k=%lld)", (long long)n, (long long)k);
     return NNCF_AMD_ERR_UNSUPPORTED;

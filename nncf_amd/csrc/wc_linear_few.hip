@@ -420,13 +420,10 @@ int few_start(const FewArgs& a, const FewShape& sh, hipStream_t s) {
     const bool gated = a.ep.act == kActSwiglu;
     const int64_t width = gated ? a.ep.n / 2 : a.ep.n, strips = (width + 15) / 16 * (gated ? 2 : 1);
     const int64_t blocks = (strips + sh.wn - 1) / sh.wn;
-    const int first = once.first_on_device();
-    if (first < 0 || (first && hipFuncSetAttribute((const void*)k_few_rows<MODE, DT, TT, XI>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                   kFewLdsBytes) != hipSuccess)) {
-        if (first > 0) once.forget_current();
-        set_error("linear: LDS refused");
-        return NNCF_AMD_ERR_LAUNCH;
-    }
+    const bool opted_in = once.run([&] {
+        return hipFuncSetAttribute((const void*)k_few_rows<MODE, DT, TT, XI>, hipFuncAttributeMaxDynamicSharedMemorySize, kFewLdsBytes) == hipSuccess;
+    });
+    if (!opted_in) return lds_refused(kFewLdsBytes);
     if (blocks > 0x7fffffff || a.rows.experts > 65535) {
         set_error("linear: weight too large");
         return NNCF_AMD_ERR_UNSUPPORTED;

@@ -862,15 +862,13 @@ static int se_step_launch(const SeStepArgs& a, int64_t batch, hipStream_t s) {
     static OncePerDevice attr_once;
     if constexpr (SeExact16<Policy>::value) {
         using SH = Se16Shape<DT, GS>;
-        if (attr_once.first_on_device() != 0) {
-            if (hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 2, true>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) != hipSuccess ||
-                hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 4, true>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) != hipSuccess ||
-                hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 2, false>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) != hipSuccess ||
-                hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 4, false>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) != hipSuccess) {
-                attr_once.forget_current();
-                return launch_status("se_step attribute");
-            }
-        }
+        const bool opted_in = attr_once.run([&] {
+            return hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 2, true>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) == hipSuccess &&
+                   hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 4, true>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) == hipSuccess &&
+                   hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 2, false>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) == hipSuccess &&
+                   hipFuncSetAttribute((const void*)k_se_step16<Policy, DT, GS, 4, false>, hipFuncAttributeMaxDynamicSharedMemorySize, SH::kBytes) == hipSuccess;
+        });
+        if (!opted_in) return launch_status("se_step attribute");
         // equal runs of tiles over one resident set of blocks (one block per CU)
         const int64_t total = a.groups * ((a.rows + 15) / 16);
         int64_t nb = 256 / batch > 0 ? 256 / batch : 1;
@@ -886,13 +884,11 @@ static int se_step_launch(const SeStepArgs& a, int64_t batch, hipStream_t s) {
             hipLaunchKernelGGL((k_se_step16<Policy, DT, GS, 4, false>), grid, block, SH::kBytes, s, a);
     } else {
         constexpr size_t lds_bytes = (size_t)se_lds_floats<GS>() * sizeof(float);
-        if (attr_once.first_on_device() != 0) {
-            if (hipFuncSetAttribute((const void*)k_se_step<Policy, DT, GS, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess ||
-                hipFuncSetAttribute((const void*)k_se_step<Policy, DT, GS, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) != hipSuccess) {
-                attr_once.forget_current();
-                return launch_status("se_step attribute");
-            }
-        }
+        const bool opted_in = attr_once.run([&] {
+            return hipFuncSetAttribute((const void*)k_se_step<Policy, DT, GS, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess &&
+                   hipFuncSetAttribute((const void*)k_se_step<Policy, DT, GS, 4>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds_bytes) == hipSuccess;
+        });
+        if (!opted_in) return launch_status("se_step attribute");
         if (a.ns <= 32)
             hipLaunchKernelGGL((k_se_step<Policy, DT, GS, 2>), grid_of(kSeWaves), dim3(kSeThreads), lds_bytes, s, a);
         else
@@ -1509,12 +1505,10 @@ extern "C" int nncf_amd_awq_prepare(const float* gscale, const float* alphas, co
     AwqPrepArgs a = {gscale, alphas, gacts, gprev, scales, sacts, (int)group_size, (int)n_samples, steps,
                      lay.tiles, lay.split ? 1 : 0, prev_s, n_prev};
     static OncePerDevice attr_once;
-    if (attr_once.first_on_device() != 0) {
-        if (hipFuncSetAttribute((const void*)k_awq_prepare, hipFuncAttributeMaxDynamicSharedMemorySize, 160000) != hipSuccess) {
-            attr_once.forget_current();
-            return launch_status("awq_prepare attribute");
-        }
-    }
+    const bool opted_in = attr_once.run([&] {
+        return hipFuncSetAttribute((const void*)k_awq_prepare, hipFuncAttributeMaxDynamicSharedMemorySize, 160000) == hipSuccess;
+    });
+    if (!opted_in) return launch_status("awq_prepare attribute");
     hipLaunchKernelGGL(k_awq_prepare, dim3((unsigned)steps, (unsigned)groups), dim3(256), (size_t)group_size * sizeof(float),
                        (hipStream_t)stream, a);
     return launch_status("awq_prepare");
