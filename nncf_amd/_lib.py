@@ -171,12 +171,12 @@ def stream_of(t: torch.Tensor):
     return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream  # what torch.cuda.current_stream(index).cuda_stream holds, without the object
 _SAME_DEVICE = contextlib.nullcontext()
 
 
 def raw_stream(t: torch.Tensor) -> int:
-    return _raw_stream(t.get_device())
+    """What torch.cuda.current_stream(t.device).cuda_stream holds, without the object (a torch without GPU support lacks it)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def on_device_of(t: torch.Tensor):
