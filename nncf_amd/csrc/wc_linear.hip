@@ -674,8 +674,8 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
         set_error("activation_grad: null or overlapping rows (ldd=%lld ldz=%lld)", (long long)ldd, (long long)ldz);
         return NNCF_AMD_ERR_BAD_ARG;
     }
-    if (chunks > 65535 || blocks > 0x7fffffff) {
-        set_error("activation_grad: too many rows");
+    if (blocks > 0x7fffffff) {
+        set_error("activation_grad: too many columns");
         return NNCF_AMD_ERR_UNSUPPORTED;
     }
     if (dbias && m > 0 && (!workspace || workspace_bytes < nncf_amd_activation_grad_workspace(m, n))) {
@@ -684,11 +684,15 @@ extern "C" int nncf_amd_activation_grad(const void* dy, int dtype, int64_t ldd, 
     }
     hipStream_t s = (hipStream_t)stream;
     float* sums = dbias ? (float*)workspace : nullptr;
-    if (m > 0 && (dz || dbias)) {
-        const dim3 grid((unsigned)blocks, (unsigned)chunks);
-#define GO(DT, VEC)                                                                                                              \
-    hipLaunchKernelGGL((k_activation_grad<DT, VEC>), grid, dim3(256), 0, s, (const uint16_t*)dy, ldd, slope, m, n, \
-                       activation, (uint16_t*)dz, ldz, sums)
+    for (int64_t c0 = 0; c0 < chunks && (dz || dbias); c0 += 65535) {  // the grid's second axis ends at 65535
+        const int64_t r0 = c0 * kChunkRows, part = chunks - c0 < 65535 ? chunks - c0 : 65535;
+        const int64_t here = m - r0 < part * kChunkRows ? m - r0 : part * kChunkRows;
+        const dim3 grid((unsigned)blocks, (unsigned)part);
+        const uint16_t* d = (const uint16_t*)dy + r0 * ldd;
+        const float* sl = slope ? slope + r0 * n : nullptr;
+        uint16_t* z = dz ? (uint16_t*)dz + r0 * ldz : nullptr;
+        float* to = sums ? sums + c0 * n : nullptr;
+#define GO(DT, VEC) hipLaunchKernelGGL((k_activation_grad<DT, VEC>), grid, dim3(256), 0, s, d, ldd, sl, here, n, activation, z, ldz, to)
         if (dtype == NNCF_AMD_BF16) {
             if (wide) GO(NNCF_AMD_BF16, 4);
             else GO(NNCF_AMD_BF16, 1);
