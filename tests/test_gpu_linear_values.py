@@ -110,3 +110,51 @@ def test_the_slope_of_gelu_is_right_to_its_last_place(m, dtype):
     off = (cdf + rest.abs()) * (40 * u + 3 * u * z * z / 2) + 2.0 ** -126 * (1 + z.abs())
     half = torch.finfo(dtype).eps / 2
     assert_within(got, want, off + (want.abs() + off) * half + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 16, 64, 256, 2048])
+@pytest.mark.parametrize("mode", ["int4_sym", "int4_asym", "nf4", "mxfp4", "int8_asym", "int8_sym"])
+def test_subnormal_weights_are_the_decompressor_s_bit_for_bit(mode, rows, dtype):
+    """x = unit rows, so a result is the weight itself: with scales of fp16's subnormal range (integer modes, NF4) or the lowest
+    bytes of E8M0, most weights are below their type's smallest normal number.  No way of the product flushes them."""
+    from nncf_amd.linear import compressed_linear
+    k, n = 256, 64
+    packed, dec = make_weight(mode, -1 if mode.startswith("int8") else 32, (n, k), dtype, seed=1)
+    if mode == "mxfp4":  # bytes 0 ... 126
+        dec._scale.copy_((torch.arange(dec._scale.numel(), device="cuda") % 127).to(torch.uint8).view_as(dec._scale))
+    else:
+        dec._scale.copy_((torch.rand(dec._scale.shape, generator=torch.Generator().manual_seed(2)) * 4e-7 + 6e-8).half())
+    w = dec(packed)
+    below = (w != 0) & (w.abs() < torch.finfo(dtype).tiny)
+    assert int(below.sum()) >= (50 if mode == "mxfp4" else n * k // 2 if dtype == torch.float16 else 0)
+    eye = torch.eye(k, dtype=dtype, device="cuda").repeat(8, 1)
+    got = torch.cat([compressed_linear(eye[r:r + rows], packed, dec) for r in range(0, max(k, rows), rows)])
+    assert torch.equal(got, w.t().repeat(8, 1)[: got.shape[0]])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 64, 256])
+def test_subnormal_activations_count(rows, dtype):
+    from nncf_amd.linear import compressed_linear
+    packed, dec = make_weight("int8_sym", -1, (64, 256), dtype, seed=1)
+    dec._scale.fill_(1.0)
+    step = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    x = torch.zeros(256, 256, dtype=dtype, device="cuda").fill_diagonal_(4 * step)
+    got = torch.cat([compressed_linear(x[r:r + rows], packed, dec) for r in range(0, 256, rows)])
+    assert torch.equal(got, (dec(packed).double().t() * 4 * step).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_subnormal_weights_in_the_gradient(dtype):
+    """dy = unit rows: dx is a row of the weight."""
+    from nncf_amd.linear import compressed_linear
+    for mode in ("int4_asym", "int8_sym", "mxfp4"):
+        packed, dec = make_weight(mode, -1 if mode == "int8_sym" else 32, (256, 64), dtype, seed=3)
+        if mode == "mxfp4":
+            dec._scale.copy_((torch.arange(dec._scale.numel(), device="cuda") % 100).to(torch.uint8).view_as(dec._scale))
+        else:
+            dec._scale.copy_((torch.rand(dec._scale.shape, generator=torch.Generator().manual_seed(4)) * 4e-7 + 6e-8).half())
+        x = torch.zeros(256, 64, dtype=dtype, device="cuda", requires_grad=True)
+        dx = torch.autograd.grad(compressed_linear(x, packed, dec), x, torch.eye(256, dtype=dtype, device="cuda"))[0]
+        assert torch.equal(dx, dec(packed))
