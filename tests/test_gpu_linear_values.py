@@ -158,3 +158,47 @@ def test_subnormal_weights_in_the_gradient(dtype):
         x = torch.zeros(256, 64, dtype=dtype, device="cuda", requires_grad=True)
         dx = torch.autograd.grad(compressed_linear(x, packed, dec), x, torch.eye(256, dtype=dtype, device="cuda"))[0]
         assert torch.equal(dx, dec(packed))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu", "swiglu"])
+@pytest.mark.parametrize("m", [1, 60, 333])
+def test_the_gradient_of_x_is_rounded_twice(m, act, dtype):
+    """Between dy and dx only dz is rounded to 16 bits (half a step), and dx itself: the slopes are those of the fp32 sums.  With u
+    = 2^-24: a sum z of K products is off by ez <= 2 (K + 2) u sum|x w|, a slope by at most 1.2 ez and by 32 u (1 + |z|) of its
+    arithmetic (swiglu: that of silu times the other half, which is off by its own ez); dz by that and half a step; dx, a sum of N
+    products, by 2 N u of their magnitudes."""
+    from nncf_amd.linear import compressed_linear
+    from tests.linear_utils import act64
+    n, k, u, half = 320, 256, 2.0 ** -24, torch.finfo(dtype).eps / 2
+    packed, dec = make_weight("int4_sym", 64, (n, k), dtype, seed=m)
+    x = (_rows(m, k, dtype, m) * 0.3).requires_grad_()
+    y = compressed_linear(x, packed, dec, activation=act)
+    dy = _rows(m, y.shape[-1], dtype, m + 2)
+    y.backward(dy)
+    w, d = dec(packed).double(), dy.double()
+    z = (x.detach().double() @ w.t()).requires_grad_()
+    dz = torch.autograd.grad(act64(z, act), z, d)[0]
+    z = z.detach()
+    ez = 2 * (k + 2) * u * (x.detach().double().abs() @ w.abs().t())
+    if act == "swiglu":
+        (a, b), (ea, eb) = z.chunk(2, -1), ez.chunk(2, -1)
+        off = torch.cat((d.abs() * (1.2 * (ea * b.abs() + eb) + 32 * u * (1 + a.abs()) * b.abs()),
+                         d.abs() * (1.2 * ea + 32 * u * (1 + a.abs()) * (1 + a.abs()))), -1)
+    else:
+        off = d.abs() * (1.2 * ez + 32 * u * (1 + z.abs()))
+        if act == "relu":  # the slope jumps where the sign of z is not settled
+            off = off + torch.where(z.abs() <= ez, d.abs(), torch.zeros_like(d))
+    step = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    off = off + half * (dz.abs() + off) + step
+    want = dz @ w
+    off = off @ w.abs() + 2 * n * u * ((dz.abs() + off) @ w.abs())
+    assert_within(x.grad, want, off + half * (want.abs() + off) + step)
+    # The same in the mean, where a slope kept in 16 bits would show (it would add another rounding of dz, half as much again to
+    # what follows): a rounding is uniform over a step of its value, step^2 / 12 in the mean square, and those of dz meet in dx
+    # independently.  Some 10^4 of them leave a few hundredths to chance; a fifth is allowed.
+    if dtype == torch.bfloat16 and act != "relu" and m > 1:
+        def step2(v):
+            return torch.exp2(2 * torch.floor(torch.log2(v.abs().clamp(min=1e-30)))) * torch.finfo(dtype).eps ** 2 / 12
+        expected = step2(dz) @ w.square() + step2(want)
+        assert (x.grad.double() - want).square().sum() <= 1.2 * expected.sum()
