@@ -158,7 +158,7 @@ def workspace_of(nbytes: int, device) -> Optional[torch.Tensor]:
 
 
 def activation_grad(dy: torch.Tensor, slope: Optional[torch.Tensor], n: int, act: int, dtype: torch.dtype, want_dz: bool, want_dbias: bool):
-    """(dz, its row stride, dbias) of the epilogue: dz = dy * slope, padded to whole steps of the product that follows."""
+    """(dz, its row stride, dbias) of the epilogue: dz = dy * slope, rounded to `dtype`, the type that the product behind it reads."""
     width = n // 2 if act == _SWIGLU else n
     dy, ldd = rows_of(dy, width)
     m = dy.shape[0]
@@ -166,13 +166,12 @@ def activation_grad(dy: torch.Tensor, slope: Optional[torch.Tensor], n: int, act
         return dy, ldd, None
     L = _lib.lib()
     copies = want_dz and act != 0  # without an activation dz is dy
-    ldz = (n + 63) // 64 * 64
-    dz = torch.empty((m, ldz), dtype=dtype, device=dy.device) if copies else None
+    dz = torch.empty((m, n), dtype=dtype, device=dy.device) if copies else None
     dbias = torch.empty(n, dtype=dtype, device=dy.device) if want_dbias else None
     ws = workspace_of(workspace_bytes("nncf_amd_activation_grad_workspace", m, n) if want_dbias else 0, dy.device)
-    _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(slope), m, n, act, ptr(dz), ldz, ptr(dbias),
+    _lib.check(L.nncf_amd_activation_grad(ptr(dy), _DTYPES[dtype], ldd, ptr(slope), m, n, act, ptr(dz), n, ptr(dbias),
                                           ptr(ws), 0 if ws is None else ws.numel(), _lib.raw_stream(dy)))
-    return (dz, ldz, dbias) if copies else (dy, ldd, dbias)
+    return (dz, n, dbias) if copies else (dy, ldd, dbias)
 
 
 def grad_input(dz: torch.Tensor, ldz: int, w: PackedWeight, offsets: Optional[torch.Tensor], dtype: torch.dtype,
