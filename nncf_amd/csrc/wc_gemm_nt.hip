@@ -129,8 +129,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void k_gemm_nt(DenseArgs g, uint32_t 
             asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b) : "memory");
     };
     constexpr int NM = FA * FB, NR = FA + FB;
-    constexpr int kSync = 1;                // MFMAs of a stage's last quarter in front of the barrier
-    constexpr int kFirst = NM - kSync - 1;  // DMA instructions of a stage that go into the last quarter before it; the rest follows
+    constexpr int kSync = 1;  // MFMAs of a stage's last quarter in front of the barrier
     op_t a0[FA], b0[FB], a1[FA], b1[FB];
     // 16 k: the MFMAs on (ca, cb) and between them the LDS reads of the next 16 k, quarter KS of the stage at (imga, imgb).
     // KS == 0 means the last quarter of the stage before: first the barrier (the stage that follows has landed, at most `OUT`

@@ -14,7 +14,6 @@ namespace wc {
 
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32v2 __attribute__((ext_vector_type(2)));
@@ -81,6 +80,7 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b) {
 }
 
 // 8 consecutive weights of one group: p0 (4-bit modes: 8 nibbles, the lower first) or p0, p1 (8 bytes) -> four pairs.
+// (The way of codes into fp16 numbers under a fixed exponent is that of Kim et al., "Who Says Elephants Can't Run", 2022.)
 // A code enters as the fp16 number 1024 + c (its bits under the exponent 0x6400) or, where it sits four bits higher, as
 // 64 + c under 0x5400 (the units there are sixteenths), which saves the shift; the difference to 1024 + z or 64 + z is
 // exact and the packed product rounds once, as the decompressor does.

@@ -154,7 +154,6 @@ __global__ __launch_bounds__(XI == 8 ? 512 : 1024, XI == 8 ? 2 : 4) void k_few_r
                 for (uint32_t i0 = threadIdx.x; i0 < all; i0 += 2 * blockDim.x) {
                     u32v4 v[2];
                     uint32_t at[2];
-                    int zat[2];
                     u32v2 zv[2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {

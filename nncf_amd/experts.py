@@ -20,8 +20,6 @@ from nncf_amd.linear import (_DTYPES, PackedWeight, activation_grad, activation_
                              rows_of, workspace_bytes, workspace_of)
 from nncf_amd.parameters import CompressWeightsMode, as_config
 
-MAX_EXPERTS, MAX_TOPK = 1024, 64
-
 
 class ExpertRouting(NamedTuple):
     """Where the tokens of one call go.  A slot is token * top_k + place; rows are the slots in the order of their experts.
