@@ -13,8 +13,8 @@
 // of the fragments, 75 vector and some 40 scalar instructions and a barrier stand one behind the other, and two waves per SIMD
 // hide half of that (with four, half the work each, the sum was the same: 172 and 186 us for 256 rows of 28672 x 8192; asking
 // for the next fragments before multiplying the last and counting slots instead of dividing gave 146).  Deeper rings change
-// nothing.  256 rows of 28672 x 8192 int4: 139 us against 270 in either neighbour; 97 of 4096 x 14336 NF4: 41 against 64 and
-// 151; 2000 rows over eight of 4096 x 14336 int4: 400 against 580 and 590.
+// nothing.  256 rows of 28672 x 8192 int4: 145 us against 284 by strips and 278 densely; 97 of 4096 x 14336 NF4: 39 against 62
+// and 151; 2000 rows over eight of 4096 x 14336 int4: 437 against 631 and 591.
 //
 // Where the tiles of y are fewer than the compute units, blocks share k: fp32 sums in the workspace, joined by join_sums.
 #include "wc_gemm.h"

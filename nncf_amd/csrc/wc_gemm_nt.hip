@@ -251,8 +251,8 @@ bool dense_reaches(int64_t n, int64_t k, int64_t ldx, int64_t sources, bool gate
     return (gated ? n : 512) * k * 2 < kMost && (gathered ? sources : 512) * ldx * 2 < kMost;
 }
 
-// 256 x 256 tiles by eight waves (1.38 PFLOP/s on 4096 x 28672 x 8192, one block per compute unit) or 128 x 128 by four (1.10,
-// two blocks): whichever needs less time in rounds of blocks, a round of the small ones costing 0.6 of one of the large ones
+// 256 x 256 tiles by eight waves (1.29 to 1.38 PFLOP/s on 4096 x 28672 x 8192, by the card; one block per compute unit) or
+// 128 x 128 by four (1.10, two blocks): whichever needs less time in rounds of blocks, a round of the small ones costing 0.6 of one of the large ones
 // (4096 x 4096 x 4096: one round of large tiles 108 us, two of small ones 125; 2047 rows: 68 us in 512 small ones, 83 in 128
 // large ones, half a round).
 template <int DT>

@@ -15,7 +15,7 @@ constexpr int64_t padded(int64_t v) { return v <= 192 ? 192 : (v + 63) / 64 * 64
 // [experts * n, kp], kp = k rounded up to 64 (192 at least), the tail zero.  Bound by the bytes (0.5-1 read, 2 written per
 // weight).  `lanes` (a power of two) threads follow a row, 8 weights each; a thread takes the same place of kDequantRows rows,
 // whose reads are requested together and whose addresses are a scalar apart.  An expert without rows is left out.
-// 28672 x 8192 int4: 101 us, 5.9 TB/s; eight NF4 experts of 28672 x 4096, groups of 32: 405 us, 6.0 TB/s.
+// 28672 x 8192 int4: 95 us, 6.2 TB/s; eight NF4 experts of 28672 x 4096, groups of 32: 401 us, 6.1 TB/s.
 constexpr int kDequantRows = 4;
 template <int MODE, int DT>
 __global__ __launch_bounds__(256) void k_dequant_rows(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void k_dequant_rows_any(const uint8_t* __restr
 // ------------------------------------------------------------------------- weight -> its transpose, for the gradient of x
 // [experts, k, np], np = n rounded up to 64 (192 at least), the tail zero: tiles of 64 x 64 turned round in LDS as pairs of
 // neighbouring n (rows padded by 4 bytes so that the columns that are written fall on different banks).  Bound by the bytes:
-// eight int4 weights of 4096 x 14336 in 292 us, 4.0 TB/s (one tile at a time 340: its reads of 32 bytes a row wait alone).
+// eight int4 weights of 4096 x 14336 in 290 us, 4.1 TB/s (one tile at a time 340: its reads of 32 bytes a row wait alone).
 constexpr int kTurns = 4;
 template <int MODE, int DT, bool ALIGNED>
 __global__ __launch_bounds__(256) void k_dequant_transposed(const uint8_t* __restrict__ codes, const void* __restrict__ scale,
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256) void k_pack_rows(const uint16_t* __restrict__ 
 // over chunks of 32 rows, which k_sum_chunks adds up in order (no atomics: the result does not depend on the schedule).
 // dz is rounded to the activations' type because the product that takes it reads 16-bit operands.
 // A thread takes VEC consecutive columns; the chunk's rows are dealt to 4 waves whose sums meet in LDS, wave 0 first.  Bound by
-// the bytes, 8 an element: 2047 x 4096 in 17 us.
+// the bytes, 8 an element: 2047 x 4096 in 15 us.
 constexpr int kChunkRows = 32;
 template <int DT, int VEC>
 __global__ __launch_bounds__(256) void k_activation_grad(const uint16_t* __restrict__ dy, int64_t ldd, const float* __restrict__ slope,
@@ -399,11 +399,20 @@ struct Need {
     CodesShape codes;
     size_t total() const { return weight + pack; }
 };
-// The time of the dense way in us: the weight decompressed (2.6 bytes an element at 6 TB/s) and multiplied
-// by 128 x 128 or 256 x 256 tiles (1 and 1.6 us for 64 k of a round of blocks, the former 0.6 where half the blocks fill it).
-// 28672 x 8192 int4, us by strips, tiles and densely: 78, 106, 250 for 64 rows; 142, 102, 258 for 128; 270, 136, 270 for 256;
-// 537, 270, 315 for 512.  Eight experts of 4096 x 14336: 397, 253, 537 for 1200 rows, 814, 525, 615 for 3000, 1520, 1005, 909
-// for 6000.
+// The time of the dense way in us: the weight decompressed (2.6 bytes an element at 6 TB/s; 8-bit codes take 3) and multiplied by
+// 128 x 128 or 256 x 256 tiles (1 and 1.6 us for 64 k of a round of blocks, the former 0.6 where half the blocks fill it).
+// Device time in us by strips, tiles and densely, all on one card, the quickest chosen but where noted:
+//   28672 x 8192      64 rows           128 rows           256 rows           512 rows           1024 rows
+//   int4, groups 128  80 110 240        152 112 240        289 145 267        549 310 325        1070 588 520
+//   int4 asymmetric   85 117 295        167 118 270        302 150 272        608 309 318        1130 620 503
+//   NF4, groups 64    89 117 249        167 116 275        311 154 276        603 316 314        1182 624 508
+//   mxfp4             77 87 258         134 91 276         244 132 269        477 265 336        934 540 491
+//   int8              77 105 257 (*)    153 112 266        312 200 288        645 424 336        1219 767 520
+//   Eight int4 experts of 4096 x 14336: 436, 322, 538 for 1200 rows; 631, 437, 591 for 2000; 828, 543, 618 for 3000; 1617, 1057,
+//   926 for 6000.
+// Over these five modes and asymmetric int8, 4096 x 4096 and 4096 x 14336 beside this weight, and twelve numbers of rows from 16 to
+// 2048, the choice is within 14 % of the quickest but (*) at 48 and 64 rows: tiles are taken where strips are 21 to 37 % quicker for
+// 8-bit codes, and strips where tiles are 18 to 20 % (NF4) and 64 % (mxfp4) quicker on 4096 x 14336.
 double dense_us(const Weight& w, int64_t rows, bool grouped) {
     auto blocks = [&](int64_t tile) { return ((w.n + tile - 1) / tile) * ((rows + tile - 1) / tile + (grouped ? (w.experts - 1) / 2 : 0)); };
     const int64_t small = blocks(128), large = blocks(256), steps = (w.k + 63) / 64;

@@ -13,10 +13,10 @@
 // and zero points, one run of memory, come to LDS at the start: a scattered load of two bytes a lane takes the load unit about
 // as many cycles as it has lanes.
 //
-// One token over 4096 x 4096 int4 takes 8.4 us (1.0 TB/s of codes: start and end), over 28672 x 8192 42 us (2.8 TB/s), 16 tokens
+// One token over 4096 x 4096 int4 takes 7.8 us (1.1 TB/s of codes: start and end), over 28672 x 8192 44 us (2.7 TB/s), 16 tokens
 // with asymmetric codes and the gate 52: bound there by the vector instructions of the conversion (13.7 clocks a weight and
-// lane, 20 us) and what a step adds to them.  Five tokens over eight mxfp4 experts of 28672 x 4096 (one instruction a pair) 80 us,
-// 4.4 TB/s of the codes that are hit.
+// lane, 20 us) and what a step adds to them.  Five tokens that hit five of eight mxfp4 experts of 28672 x 4096 (one instruction a
+// pair) 85 us, 3.4 TB/s of the codes that are hit; seven of them 108 us, 3.8.
 #include <type_traits>
 
 #include "wc_linear.h"

@@ -181,7 +181,8 @@ def expert_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, routing: 
               (what another `expert_linear` returned)
     returns   [tokens * top_k, out] (swiglu: out / 2) in the order of the rows; rows that no token has are zero
 
-    Activations, types and gradients as in `nncf_amd.linear.compressed_linear`; differentiable in x."""
+    Activations, types and gradients as in `nncf_amd.linear.compressed_linear`; differentiable in x.  The workspace of many rows
+    or of x's gradient is two bytes per weight of the whole stack."""
     what = "expert_linear"
     _lib.require_gpu(x, what)
     refuse_transforms(what, x)

@@ -239,8 +239,10 @@ def compressed_linear(x: torch.Tensor, packed: torch.Tensor, decompressor, bias:
                  silu(gate) * up has out_features / 2 columns
     residual     the result's shape and type
 
-    Differentiable in x, bias and residual (in reverse mode, not twice); the weight is frozen.  With an activation the backward pass keeps its
-    slope at every sum, in fp32."""
+    Differentiable in x, bias and residual (in reverse mode, not twice); the weight is frozen.  With an activation the backward
+    pass keeps its slope at every sum, in fp32 (4 bytes for each of rows x out_features); the gradient of the sums is rounded to
+    x's type for the product that gives x's, as autograd's would be, so that one carries two roundings.  From some hundreds of
+    rows on, and for x's gradient, a call takes a workspace of two bytes per weight."""
     what = "compressed_linear"
     _lib.require_gpu(x, what)
     refuse_transforms(what, x, bias, residual)
