@@ -46,12 +46,21 @@ _MODE_OF = {dcmp.INT8AsymmetricWeightsDecompressor: "int8_asym", dcmp.INT8Symmet
             dcmp.NF4WeightsDecompressor: "nf4", dcmp.MXFP4WeightsDecompressor: "mxfp4"}
 
 
-def _mode_of(decompressor) -> str:
+def _mode_or_none(decompressor) -> Optional[str]:
+    """The mode whose codes `decompressor` decompresses as this package does; None for another's, also of a subclass that overrides
+    its forward (the weight would not be the one that the kernels multiply by)."""
     mode = _MODE_OF.get(type(decompressor))
     if mode is None:
         for cls, mode in _MODE_OF.items():
             if isinstance(decompressor, cls):
-                return mode
+                return mode if type(decompressor).forward is cls.forward else None
+        return None
+    return mode
+
+
+def _mode_of(decompressor) -> str:
+    mode = _mode_or_none(decompressor)
+    if mode is None:
         raise InternalError(f"{type(decompressor).__name__} is not a decompressor of this package")
     return mode
 
@@ -272,13 +281,16 @@ _LINEAR_FORWARD = nn.Linear.forward
 
 
 def _only_decompressed(mod: nn.Module):
-    """The parametrizations of `mod`'s weight if a decompressor is all they are (an adapter may have joined it, or left) and its
-    scales are as it was made with them (`model.float()` casts them), else None."""
+    """The parametrizations of `mod`'s weight if a decompressor of this package is all they are (an adapter may have joined it, or
+    left), as it was made: no hooks, nor scales that were cast (`model.float()` does).  Else None."""
     parametrizations = mod._modules.get("parametrizations")
     plist = None if parametrizations is None else parametrizations._modules.get("weight")
-    if plist is None or len(plist) != 1 or not isinstance(plist[0], dcmp.BaseWeightsDecompressor):
+    if plist is None or len(plist) != 1:
         return None
-    return plist if plist[0]._buffers["_scale"].dtype in (torch.float16, torch.uint8) else None
+    dec = plist[0]
+    if _mode_or_none(dec) is None or dec._forward_hooks or dec._forward_pre_hooks or "forward" in dec.__dict__:
+        return None
+    return plist if dec._buffers["_scale"].dtype in (torch.float16, torch.uint8) else None
 
 
 def _fused_forward(self, x: torch.Tensor) -> torch.Tensor:

@@ -1,5 +1,5 @@
 """CPU: which modules of a compressed model `fuse_compressed_linears` takes over, and when their forward hands a call back.  The
-decompressor here decompresses on the CPU; `compressed_linear` is not reached (its arguments are on no GPU)."""
+decompressors run on the CPU here; `compressed_linear` is not reached (its arguments are on no GPU)."""
 import copy
 
 import pytest
@@ -10,17 +10,20 @@ from torch.nn.utils import parametrize
 from nncf_amd import decompressors as dcmp
 
 
-class _OnCpu(dcmp.INT8SymmetricWeightsDecompressor):
-    def forward(self, x):
-        return (x.to(torch.float16) * self._scale).to(self.result_dtype)
+@pytest.fixture(autouse=True)
+def decompressed_on_the_cpu(monkeypatch):
+    def decompress(codes, mode, n_groups, group_size, scale, zero_point, out_dtype, scale_kind=None):
+        assert mode == "int8_sym"
+        return (codes.to(torch.float16).view(n_groups, group_size) * scale.view(-1, 1)).to(out_dtype).flatten()
+    monkeypatch.setattr(dcmp, "decompress", decompress)
 
 
-def _compressed(mod, seed=0):
+def _compressed(mod, seed=0, cls=dcmp.INT8SymmetricWeightsDecompressor):
     """`mod`, an nn.Linear, with its weight as int8 codes behind a decompressor."""
     g = torch.Generator().manual_seed(seed)
     codes = torch.randint(-128, 128, mod.weight.shape, dtype=torch.int8, generator=g)
     mod.weight = nn.Parameter(codes, requires_grad=False)
-    dec = _OnCpu(torch.rand(codes.shape[0], 1, generator=g) * 0.01 + 0.001, result_dtype=torch.bfloat16)
+    dec = cls(torch.rand(codes.shape[0], 1, generator=g) * 0.01 + 0.001, result_dtype=torch.bfloat16)
     parametrize.register_parametrization(mod, "weight", dec, unsafe=True)
     return mod.requires_grad_(False)
 
@@ -140,3 +143,50 @@ def test_scales_that_were_cast_keep_the_library_product(reached):
     assert torch.equal(mod(_x().as_subclass(_AsOnGpu)).as_subclass(torch.Tensor), want) and not reached
     plain = dcmp.INT8SymmetricWeightsDecompressor(torch.ones(8, 1))
     assert weight_dtype_of(plain) == torch.float16 and weight_dtype_of(plain.float()) == torch.float32
+
+
+class _Doubled(dcmp.INT8SymmetricWeightsDecompressor):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+class _Other(dcmp.BaseWeightsDecompressor):
+    result_dtype = torch.bfloat16
+
+    def __init__(self, scale, result_dtype):
+        super().__init__()
+
+    def forward(self, x):
+        return x.to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("cls", [_Doubled, _Other])
+def test_a_decompressor_with_a_forward_of_its_own_keeps_it(cls, reached):
+    from nncf_amd.linear import fuse_compressed_linears
+    torch.manual_seed(0)
+    mod = _compressed(nn.Linear(16, 8, dtype=torch.bfloat16), cls=cls)
+    want = mod(_x())
+    assert fuse_compressed_linears(mod) == 0
+    assert torch.equal(mod(_x().as_subclass(_AsOnGpu)).as_subclass(torch.Tensor), want) and not reached
+
+
+def test_hooks_of_a_decompressor_run(reached):
+    from nncf_amd.linear import fuse_compressed_linears
+    mod = _linear()
+    plain = mod(_x())
+    fuse_compressed_linears(mod)
+    handle = mod.parametrizations.weight[0].register_forward_hook(lambda m, args, out: 2 * out)
+    want = nn.functional.linear(_x(), mod.weight, mod.bias)
+    assert torch.equal(mod(_x().as_subclass(_AsOnGpu)).as_subclass(torch.Tensor), want) and not reached and not torch.equal(want, plain)
+    handle.remove()
+    assert torch.equal(mod(_x().as_subclass(_AsOnGpu)), plain) and len(reached) == 1
+
+
+def test_the_product_refuses_a_decompressor_with_a_forward_of_its_own():
+    from nncf_amd.errors import InternalError
+    from nncf_amd.linear import packed_weight
+    codes, x = torch.ones(8, 16, dtype=torch.int8), torch.ones(3, 16, dtype=torch.bfloat16)
+    kind = type("_Named", (dcmp.INT8SymmetricWeightsDecompressor,), {})
+    assert packed_weight(codes, kind(torch.ones(8, 1), torch.bfloat16), x, 2, "here").k == 16
+    with pytest.raises(InternalError):
+        packed_weight(codes, _Doubled(torch.ones(8, 1), torch.bfloat16), x, 2, "here")

@@ -7,7 +7,7 @@ import torch.autograd.forward_ad as fwd
 from nncf_amd import _lib
 from nncf_amd import decompressors as dcmp
 from nncf_amd.errors import InternalError
-from tests.test_linear_models_cpu import _AsOnGpu, _linear, _x, reached  # noqa: F401
+from tests.test_linear_models_cpu import _AsOnGpu, _linear, _x, decompressed_on_the_cpu, reached  # noqa: F401
 
 
 @pytest.fixture
